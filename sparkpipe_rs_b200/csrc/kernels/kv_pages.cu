@@ -1,0 +1,423 @@
+// Pages of a paged KV cache that several sequences share, sm_100a.
+//
+// A block table [rows][cols] holds the page of every `block_size` tokens of a row, -1
+// where it has none; refs[p] counts the table entries that hold page p (0: free). The
+// cache is one or two planes (rows of values; the fp8 cache's block scales), each
+// [layers][pages][page bytes] with any layer stride.
+//
+//  * pages_fork     — new row i continues row parents[i]: its pages are shared, the old
+//                     rows give theirs up; counts move by integer atomics, whose order
+//                     does not matter.
+//  * pages_reserve  — room for more tokens in every row, from the lowest free pages, and a
+//                     private copy of a last page that other rows hold too.
+//  * pages_free     — chosen rows give their pages back.
+//  * pages_compact  — live pages move to the front: the j-th live page behind the first
+//                     `live` ones moves to the j-th free page among them.
+//  * pages_copy     — the data movement of all of them: (source, destination) pairs over
+//                     every layer and plane.
+//
+// The index kernels run in one CTA where an order is needed (which row gets which page):
+// tables and counts are a few KB. The copies are bound by memory: every thread keeps four
+// 16-byte loads in flight, and the work is cut into 16 KB pieces so that one page of one
+// layer already spreads over several SMs.
+//
+// Reference: the page / block-table bookkeeping of the KV arena
+// (crates/spark-abi/vendor/sparkpipe/include/sparkpipe/spark_kv_cache.h:227-300); sharing
+// between live sequences is this framework's own.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <stdexcept>
+
+#include "common.cuh"
+#include "launch.h"
+#include "pdl.h"
+
+namespace sp {
+
+namespace {
+
+constexpr int kCopyThreads = 256;
+constexpr int kPiece = 4 * kCopyThreads;  // vectors of one piece: four per thread
+constexpr int kIndexThreads = 1024;
+
+// Exclusive prefix sum of one value per thread over the CTA; every thread gets the total.
+SP_DEVI int block_scan(int v, int* total, int* warp_sums) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the previous scan's readers are done with warp_sums
+  if (lane == 31) warp_sums[w] = x;
+  __syncthreads();
+  int base = 0, all = 0;
+  for (int i = 0; i < warps; ++i) {
+    const int t = warp_sums[i];
+    if (i < w) base += t;
+    all += t;
+  }
+  *total = all;
+  return base + x - v;
+}
+
+SP_DEVI int pages_of(int tokens, int block_size) { return tokens <= 0 ? 0 : (tokens - 1) / block_size + 1; }
+
+}  // namespace
+
+// ------------------------------------------------------------------ fork
+// CTAs [0, rows): old row b gives its pages up; CTAs [rows, rows + n): new row i.
+__global__ void __launch_bounds__(128) pages_fork_kernel(const int* __restrict__ table, int rows, int cols,
+                                                         const int* __restrict__ lens, const int* __restrict__ parents,
+                                                         int* __restrict__ refs, int pages, int block_size,
+                                                         int* __restrict__ new_table, int* __restrict__ new_lens) {
+  griddep_wait();
+  griddep_launch();
+  if (blockIdx.x < rows) {
+    const int* t = table + (long long)blockIdx.x * cols;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      const int e = t[c];
+      if (e >= 0 && e < pages) atomicSub(refs + e, 1);
+    }
+    return;
+  }
+  const int i = blockIdx.x - rows;
+  const int p = parents[i];
+  const bool there = p >= 0 && p < rows;
+  const int len = there ? lens[p] : 0;
+  const int held = pages_of(len, block_size);
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    const int e = c < held ? table[(long long)p * cols + c] : -1;
+    new_table[(long long)i * cols + c] = e;
+    if (e >= 0 && e < pages) atomicAdd(refs + e, 1);
+  }
+  if (threadIdx.x == 0) new_lens[i] = len;
+}
+
+void pages_fork(const int* table, int rows, int cols, const int* lens, const int* parents, int n, int* refs, int pages,
+                int block_size, int* new_table, int* new_lens, cudaStream_t s) {
+  if (rows + n <= 0) return;
+  launch_k(pages_fork_kernel, dim3((unsigned)(rows + n)), dim3(128), 0, s, table, rows, cols, lens, parents, refs,
+           pages, block_size, new_table, new_lens);
+}
+
+// ------------------------------------------------------------------ reserve
+// One CTA. Phase 1: what each row needs, and its place among the needs of the rows before
+// it; phase 2: the lowest free pages, as many as are needed; phase 3: grants. `free_list`
+// holds [pages] ids; `work` gets the copy list, (source, destination, tokens) records, and
+// `copies` its length.
+__global__ void __launch_bounds__(kIndexThreads)
+    pages_reserve_kernel(int* __restrict__ table, int rows, int cols, const int* __restrict__ lens,
+                         const int* __restrict__ row_tokens, int tokens, int* __restrict__ refs, int pages,
+                         int block_size, int* __restrict__ free_list, int* __restrict__ work, int* __restrict__ copies,
+                         int* __restrict__ short_by) {
+  extern __shared__ int smem[];
+  int* tail = smem;          // [rows] last page if other rows hold it too, else -1
+  int* start = smem + rows;  // [rows] pages granted to the rows before
+  int* need = start + rows;  // [rows]
+  __shared__ int warp_sums[32];
+  __shared__ int s_copies;
+  griddep_wait();
+  griddep_launch();
+  if (threadIdx.x == 0) s_copies = 0;
+  for (int b = threadIdx.x; b < rows; b += blockDim.x) {
+    const int len = lens[b];
+    const int want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
+    int t = -1;
+    if (want > 0 && len > 0 && len % block_size != 0 && len / block_size < cols) {
+      t = table[(long long)b * cols + len / block_size];
+      if (t < 0 || t >= pages || refs[t] <= 1) t = -1;
+    }
+    tail[b] = t;
+  }
+  __syncthreads();
+  int carry = 0;
+  for (int b0 = 0; b0 < rows; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    int n = 0;
+    if (b < rows) {
+      const int len = max(lens[b], 0);
+      const int want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
+      const int t = tail[b];
+      if (t >= 0) {
+        int earlier = 0;
+        for (int q = 0; q < b; ++q) earlier += tail[q] == t;
+        if (refs[t] - earlier > 1) n = 1;
+      }
+      if (want > 0) {
+        const long long end = (long long)len + want;
+        const int first = pages_of(len, block_size);
+        const int last = int(min((long long)cols, (end - 1) / block_size + 1));
+        for (int c = first; c < last; ++c) n += table[(long long)b * cols + c] < 0;
+      }
+      need[b] = n;
+    }
+    int total;
+    const int at = block_scan(b < rows ? n : 0, &total, warp_sums);
+    if (b < rows) start[b] = carry + at;
+    carry += total;
+  }
+  // free pages, lowest first
+  int found = 0;
+  for (int p0 = 0; p0 < pages && found < carry; p0 += blockDim.x) {
+    const int p = p0 + threadIdx.x;
+    const int is_free = p < pages && refs[p] <= 0;
+    int total;
+    const int at = found + block_scan(is_free, &total, warp_sums);
+    if (is_free && at < carry) free_list[at] = p;
+    found += total;
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < rows; b += blockDim.x) {
+    const int n = need[b];
+    const bool served = n > 0 && start[b] + n <= found;
+    short_by[b] = served ? 0 : n;
+    if (!served) continue;
+    const int len = max(lens[b], 0);
+    const int want = row_tokens ? row_tokens[b] : tokens;
+    int g = start[b];
+    int* t = table + (long long)b * cols;
+    const int first = pages_of(len, block_size);
+    const int last = int(min((long long)cols, ((long long)len + want - 1) / block_size + 1));
+    int fresh = 0;
+    for (int c = first; c < last; ++c) fresh += t[c] < 0;
+    if (n > fresh) {  // the shared last page comes first
+      const int page = free_list[g++];
+      const int i = atomicAdd(&s_copies, 1);
+      int* rec = work + 3 * i;
+      rec[0] = tail[b];
+      rec[1] = page;
+      rec[2] = len % block_size;
+      atomicSub(refs + tail[b], 1);
+      refs[page] = 1;
+      t[len / block_size] = page;
+    }
+    for (int c = first; c < last; ++c)
+      if (t[c] < 0) {
+        const int page = free_list[g++];
+        refs[page] = 1;
+        t[c] = page;
+      }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *copies = s_copies;
+}
+
+void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, int* refs,
+                   int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s) {
+  if (rows <= 0) return;
+  if (rows > kPagesMaxRows) throw std::runtime_error("pages_reserve: too many rows");
+  launch_k(pages_reserve_kernel, dim3(1), dim3(kIndexThreads), sizeof(int) * 3 * rows, s, table, rows, cols, lens,
+           row_tokens, tokens, refs, pages, block_size, free_list, work, copies, short_by);
+}
+
+// ------------------------------------------------------------------ free
+__global__ void __launch_bounds__(128) pages_free_kernel(int* __restrict__ table, int cols, int* __restrict__ refs,
+                                                         int pages, const int* __restrict__ rows, int n) {
+  griddep_wait();
+  griddep_launch();
+  const int b = blockIdx.x;
+  if (rows) {  // a row that is named twice is freed once
+    int named = 0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) named |= rows[i] == b;
+    if (!__syncthreads_or(named)) return;
+  }
+  int* t = table + (long long)b * cols;
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    const int e = t[c];
+    if (e >= 0 && e < pages) atomicSub(refs + e, 1);
+    t[c] = -1;
+  }
+}
+
+void pages_free(int* table, int rows, int cols, int* refs, int pages, const int* which, int n, cudaStream_t s) {
+  if (rows <= 0) return;
+  launch_k(pages_free_kernel, dim3((unsigned)rows), dim3(128), 0, s, table, cols, refs, pages, which, n);
+}
+
+// ------------------------------------------------------------------ compact
+// One CTA: live pages are counted, then the free pages below that count and the live ones
+// at or above it are listed in order (equally many) and paired. `work`: [pages] x (source,
+// destination, tokens) pairs; `holes` [pages].
+__global__ void __launch_bounds__(kIndexThreads)
+    pages_compact_kernel(int* __restrict__ refs, int pages, int block_size, int* __restrict__ page_map,
+                         int* __restrict__ live_out, int* __restrict__ work, int* __restrict__ holes,
+                         int* __restrict__ copies) {
+  __shared__ int warp_sums[32];
+  griddep_wait();
+  griddep_launch();
+  int mine = 0, live, total;
+  for (int p = threadIdx.x; p < pages; p += blockDim.x) mine += refs[p] > 0;
+  block_scan(mine, &live, warp_sums);
+  int n_holes = 0;
+  for (int p0 = 0; p0 < live; p0 += blockDim.x) {
+    const int p = p0 + threadIdx.x;
+    const int hole = p < live && refs[p] <= 0;
+    const int at = n_holes + block_scan(hole, &total, warp_sums);
+    if (hole) holes[at] = p;
+    if (p < live) page_map[p] = hole ? -1 : p;
+    n_holes += total;
+  }
+  __syncthreads();
+  int moved = 0;
+  for (int p0 = live; p0 < pages; p0 += blockDim.x) {
+    const int p = p0 + threadIdx.x;
+    const int r = p < pages ? refs[p] : 0;
+    const int moves = r > 0;
+    const int at = moved + block_scan(moves, &total, warp_sums);
+    if (moves) {
+      const int to = holes[at];
+      work[3 * at] = p;
+      work[3 * at + 1] = to;
+      work[3 * at + 2] = block_size;
+      page_map[p] = to;
+      refs[to] = r;
+      refs[p] = 0;
+    } else if (p < pages) {
+      page_map[p] = -1;
+    }
+    moved += total;
+  }
+  if (threadIdx.x == 0) {
+    *copies = moved;
+    *live_out = live;
+  }
+}
+
+void pages_compact(int* refs, int pages, int block_size, int* page_map, int* live, int* work, int* holes, int* copies,
+                   cudaStream_t s) {
+  launch_k(pages_compact_kernel, dim3(1), dim3(kIndexThreads), 0, s, refs, pages, block_size, page_map, live, work,
+           holes, copies);
+}
+
+// ------------------------------------------------------------------ copy
+// Checks a caller's (source, destination) pairs and writes the copy list. A pair with -1,
+// or of a page with itself, is skipped. Pairs whose order would matter (a page that is
+// the destination of two pairs, or the destination of one and the source of another), and
+// pages outside the cache, refuse the whole call: nothing is copied and the status word is
+// set. `marks`: a bit per page in shared memory.
+__global__ void __launch_bounds__(kIndexThreads)
+    pages_pairs_kernel(const int* __restrict__ src, const int* __restrict__ dst, int n, int pages, int block_size,
+                       int* __restrict__ work, int* __restrict__ copies, int* err) {
+  extern __shared__ int smem[];
+  unsigned* marks = reinterpret_cast<unsigned*>(smem);
+  __shared__ int s_count;
+  griddep_wait();
+  griddep_launch();
+  for (int i = threadIdx.x; i < (pages + 31) / 32; i += blockDim.x) marks[i] = 0;
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+  int bad = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int a = src[i], b = dst[i];
+    if (a == -1 || b == -1) continue;
+    if (a < 0 || b < 0 || a >= pages || b >= pages) { bad = 1; continue; }
+    if (a == b) continue;
+    if (atomicOr(&marks[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) bad = 1;
+  }
+  bad = __syncthreads_or(bad);
+  for (int i = threadIdx.x; i < n && !bad; i += blockDim.x) {
+    const int a = src[i], b = dst[i];
+    if (a == -1 || b == -1 || a == b) continue;
+    if (marks[a >> 5] & (1u << (a & 31))) bad = 1;
+    const int at = atomicAdd(&s_count, 1);
+    work[3 * at] = a;
+    work[3 * at + 1] = b;
+    work[3 * at + 2] = block_size;
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) {
+    *copies = bad ? 0 : s_count;
+    if (bad && err) atomicCAS(err, 0, kErrBadIndex);
+  }
+}
+
+void pages_pairs(const int* src, const int* dst, int n, int pages, int block_size, int* work, int* copies, int* err,
+                 cudaStream_t s) {
+  if (pages > kPagesMaxMarked) throw std::runtime_error("copy_pages: too many pages");
+  const size_t bytes = sizeof(int) * ((pages + 31) / 32);
+  set_smem_bytes(pages_pairs_kernel, kPagesMaxMarked / 8);
+  launch_k(pages_pairs_kernel, dim3(1), dim3(kIndexThreads), bytes, s, src, dst, n, pages, block_size, work, copies,
+           err);
+}
+
+struct CopyPlane {
+  char* base;
+  long long layer_stride;  // bytes
+  int page_bytes, token_bytes, pieces;
+};
+
+// Persistent CTAs over (pair, layer, piece) units, pieces of both planes one after the
+// other. V is the access width: 16 bytes, or 4 where a plane's addresses are only that
+// aligned. A pair's token count bounds its bytes (a last page is copied as far as its row
+// has tokens). The first threads also pass a table through the page map of a compaction.
+template <typename V>
+__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const int* __restrict__ work,
+                                                                  const int* __restrict__ copies, int layers,
+                                                                  CopyPlane a, CopyPlane b, int* __restrict__ table,
+                                                                  long long entries, const int* __restrict__ page_map,
+                                                                  int pages) {
+  griddep_wait();
+  griddep_launch();
+  if (table)
+    for (long long i = (long long)blockIdx.x * kCopyThreads + threadIdx.x; i < entries;
+         i += (long long)gridDim.x * kCopyThreads) {
+      const int e = table[i];
+      if (e >= 0 && e < pages) table[i] = page_map[e];
+    }
+  const int per_page = a.pieces + b.pieces;
+  const long long units = (long long)*copies * layers * per_page;
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int piece = int(u % per_page);
+    const long long q = u / per_page;
+    const int layer = int(q % layers), i = int(q / layers);
+    const CopyPlane& pl = piece < a.pieces ? a : b;
+    const int src = work[3 * i], dst = work[3 * i + 1];
+    const int bytes = work[3 * i + 2] * pl.token_bytes;
+    const int v0 = (piece < a.pieces ? piece : piece - a.pieces) * kPiece + threadIdx.x;
+    const char* from = pl.base + layer * pl.layer_stride + (long long)src * pl.page_bytes;
+    char* to = pl.base + layer * pl.layer_stride + (long long)dst * pl.page_bytes;
+    const int whole = bytes / (int)sizeof(V);
+    V v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v0 + j * kCopyThreads < whole) v[j] = reinterpret_cast<const V*>(from)[v0 + j * kCopyThreads];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = v0 + j * kCopyThreads;
+      if (at < whole) {
+        reinterpret_cast<V*>(to)[at] = v[j];
+      } else if (at == whole) {  // the words of a token count that does not fill a vector
+        for (int w = whole * (int)sizeof(V); w < bytes; w += 4)
+          *reinterpret_cast<int*>(to + w) = *reinterpret_cast<const int*>(from + w);
+      }
+    }
+  }
+}
+
+void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_size, const int* work, const int* copies,
+                long long max_copies, int* table, long long entries, const int* page_map, int pages, int num_sms,
+                cudaStream_t s) {
+  bool wide = true;
+  auto plane = [&](const PagePlane& p) {
+    CopyPlane c = {static_cast<char*>(p.base), p.layer_stride, p.token_bytes * block_size, p.token_bytes, 0};
+    if (p.base && ((reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.layer_stride | (uintptr_t)c.page_bytes) & 15)) wide = false;
+    return c;
+  };
+  CopyPlane ca = plane(a), cb = plane(b);
+  const int vec = wide ? 16 : 4;
+  for (CopyPlane* c : {&ca, &cb}) c->pieces = c->base ? (c->page_bytes / vec + kPiece - 1) / kPiece : 0;
+  const long long units = max_copies * layers * (ca.pieces + cb.pieces);
+  const long long remap = (entries + kCopyThreads - 1) / kCopyThreads;
+  const long long want = std::max(units, table ? remap : 0ll);
+  if (want <= 0) return;
+  const int grid = (int)std::min<long long>(want, 8ll * num_sms);
+  if (wide) launch_k(pages_copy_kernel<uint4>, dim3(grid), dim3(kCopyThreads), 0, s, work, copies, layers, ca, cb, table,
+                     entries, page_map, pages);
+  else launch_k(pages_copy_kernel<int>, dim3(grid), dim3(kCopyThreads), 0, s, work, copies, layers, ca, cb, table,
+                entries, page_map, pages);
+}
+
+}  // namespace sp

@@ -323,6 +323,33 @@ void spec_finish(int* tok_rows, const int* tgt_rows, int B, int L, float p_accep
 // Paged KV blocks of a [layers][slots][row] bf16 cache <-> staging [n][layers][block_size][row].
 void kv_blocks_copy(void* cache, long long layer_stride, const int* blocks, int n, void* staging, int layers,
                     int block_size, int row, int to_staging, cudaStream_t s);
+// Log probabilities, entropy and the k most probable tokens of logits rows (logprobs.cu);
+// dtype 0 bf16, 1 fp16, 2 fp32; ids [rows, given].
+constexpr int kLogprobsMaxTop = 32;
+void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,
+                    float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s);
+// Pages of a paged cache shared by several sequences (kv_pages.cu). A plane is [layers][pages][page
+// bytes] with `layer_stride` bytes between layers (base null: no plane). `work` holds (source,
+// destination, tokens) records, `copies` their number.
+constexpr int kPagesMaxRows = 4000;            // rows of one pages_reserve call (shared memory)
+constexpr int kPagesMaxMarked = 8 * 128 * 1024;  // pages of one pages_pairs call (a bit each in shared memory)
+struct PagePlane {
+  void* base = nullptr;
+  long long layer_stride = 0;
+  int token_bytes = 0;
+};
+void pages_fork(const int* table, int rows, int cols, const int* lens, const int* parents, int n, int* refs, int pages,
+                int block_size, int* new_table, int* new_lens, cudaStream_t s);
+void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, int* refs,
+                   int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s);
+void pages_free(int* table, int rows, int cols, int* refs, int pages, const int* which, int n, cudaStream_t s);
+void pages_compact(int* refs, int pages, int block_size, int* page_map, int* live, int* work, int* holes, int* copies,
+                   cudaStream_t s);
+void pages_pairs(const int* src, const int* dst, int n, int pages, int block_size, int* work, int* copies, int* err,
+                 cudaStream_t s);
+void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_size, const int* work, const int* copies,
+                long long max_copies, int* table, long long entries, const int* page_map, int pages, int num_sms,
+                cudaStream_t s);
 // Phase clocks: totals[slot] += now - stamps[prev] (prev >= 0); stamps[slot] <- device global timer (ns).
 void phase_mark(unsigned long long* stamps, unsigned long long* totals, int slot, int prev, cudaStream_t s);
 void decode_advance(const int* out_ids, int* ids, int* pos, int* ctx, int* slots, const int* block_table,

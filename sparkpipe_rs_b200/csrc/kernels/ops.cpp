@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <climits>
 #include <cstring>
 #include <mutex>
 #include <unordered_map>
@@ -1088,6 +1089,185 @@ void ep_advance(const Tensor& epoch) {
   sp::ep_advance(epoch.data_ptr<int64_t>(), stream());
 }
 
+// ---- log probabilities and shared cache pages
+void token_logprobs(const Tensor& logits, const Tensor& ids, const Tensor& lp, const Tensor& entropy,
+                    const Tensor& top_lp, const Tensor& top_ids) {
+  TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
+              "token_logprobs: logits must be [T, V] with unit column stride");
+  const auto st = logits.scalar_type();
+  TORCH_CHECK(st == at::kBFloat16 || st == at::kHalf || st == at::kFloat,
+              "token_logprobs: logits must be bf16, fp16 or fp32");
+  const int64_t T = logits.size(0), V = logits.size(1), k = top_lp.size(1);
+  TORCH_CHECK(T == 0 || V >= 1, "token_logprobs: no columns");
+  TORCH_CHECK(T <= INT_MAX && V <= INT_MAX - 4096, "token_logprobs: too large");
+  CHECK_I32(ids); CHECK_CONTIG(ids);
+  TORCH_CHECK((ids.dim() == 1 || ids.dim() == 2) && ids.size(0) == T,
+              "token_logprobs: ids must be [T] or [T, n], one row per logits row");
+  const int64_t given = ids.dim() == 2 ? ids.size(1) : 1;
+  TORCH_CHECK(k >= 0 && k <= sp::kLogprobsMaxTop && (T == 0 || k <= V),
+              "token_logprobs: top_k must be between 0 and min(" + std::to_string(sp::kLogprobsMaxTop) + ", V)");
+  CHECK_F32(lp); CHECK_F32(entropy); CHECK_F32(top_lp); CHECK_I32(top_ids);
+  CHECK_CONTIG(lp); CHECK_CONTIG(entropy); CHECK_CONTIG(top_lp); CHECK_CONTIG(top_ids);
+  TORCH_CHECK(lp.numel() == ids.numel() && entropy.numel() == T && top_lp.numel() == T * k &&
+              top_ids.numel() == T * k, "token_logprobs: output shapes");
+  CHECK_CUDA(logits); CHECK_ON(logits, ids); CHECK_ON(logits, lp); CHECK_ON(logits, entropy);
+  CHECK_ON(logits, top_lp); CHECK_ON(logits, top_ids);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  sp::token_logprobs(logits.data_ptr(), st == at::kBFloat16 ? 0 : st == at::kHalf ? 1 : 2, logits.stride(0), (int)T,
+                     (int)V, ids.data_ptr<int>(), (int)given, (int)k, lp.data_ptr<float>(), entropy.data_ptr<float>(),
+                     top_lp.data_ptr<float>(), top_ids.data_ptr<int>(), stream());
+}
+
+// One plane of a paged cache [layers, slots, row]; any layer stride, rows and slots dense.
+sp::PagePlane page_plane(const Tensor& t, int64_t block_size, const char* who) {
+  TORCH_CHECK(t.dim() == 3 && t.size(2) >= 1 && (t.stride(2) == 1 || t.size(2) == 1) &&
+              (t.stride(1) == t.size(2) || t.size(1) <= 1),
+              who, ": the cache must be [layers, slots, row] with dense slots");
+  TORCH_CHECK(block_size >= 1 && t.size(1) % block_size == 0, who, ": slots must be whole pages");
+  const int64_t e = t.element_size(), token = t.size(2) * e;
+  TORCH_CHECK(token % 4 == 0 && (t.stride(0) * e) % 4 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 3) == 0,
+              who, ": cache rows must be whole 4-byte words");
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1) * t.size(2), who, ": cache layers overlap");
+  TORCH_CHECK(token * block_size < (int64_t(1) << 30), who, ": pages of 1 GiB or more");
+  sp::PagePlane p;
+  p.base = t.data_ptr();
+  p.layer_stride = t.stride(0) * e;
+  p.token_bytes = (int)token;
+  return p;
+}
+
+// Both planes of a cache; returns its pages.
+int64_t page_planes(const Tensor& data, const c10::optional<Tensor>& scales, int64_t block_size, sp::PagePlane* a,
+                    sp::PagePlane* b, const char* who) {
+  *a = page_plane(data, block_size, who);
+  if (scales.has_value()) {
+    TORCH_CHECK(scales->dim() == 3 && scales->size(0) == data.size(0) && scales->size(1) == data.size(1),
+                who, ": cache_scales must have the cache's layers and slots");
+    *b = page_plane(*scales, block_size, who);
+    CHECK_ON(data, *scales);
+  }
+  const int64_t pages = data.size(1) / block_size;
+  TORCH_CHECK(pages <= sp::kPagesMaxMarked && data.size(0) <= INT_MAX, who, ": too many pages");
+  return pages;
+}
+
+void check_page_table(const Tensor& table, const Tensor& refs, const char* who) {
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous(),
+              who, ": block_table must be contiguous int32 [rows, columns]");
+  TORCH_CHECK(refs.scalar_type() == at::kInt && refs.dim() == 1 && refs.is_contiguous() && refs.numel() >= 1,
+              who, ": refs must be contiguous int32 [pages]");
+  TORCH_CHECK(table.size(0) <= INT_MAX / 2 && table.size(1) <= INT_MAX / 2 && refs.numel() <= sp::kPagesMaxMarked,
+              who, ": too large");
+}
+
+int64_t copy_pages(const Tensor& data, const c10::optional<Tensor>& scales, const Tensor& src, const Tensor& dst,
+                   int64_t block_size) {
+  sp::PagePlane a, b;
+  CHECK_I32(src); CHECK_I32(dst); CHECK_CONTIG(src); CHECK_CONTIG(dst);
+  TORCH_CHECK(src.dim() == 1 && dst.dim() == 1 && src.numel() == dst.numel() && src.numel() <= INT_MAX / 3,
+              "copy_pages: src and dst must be [n], a source for every destination");
+  const int64_t pages = page_planes(data, scales, block_size, &a, &b, "copy_pages");
+  CHECK_CUDA(data); CHECK_ON(data, src); CHECK_ON(data, dst);
+  const int64_t n = src.numel();
+  if (n == 0 || data.numel() == 0) return 0;
+  const c10::cuda::CUDAGuard guard(data.device());
+  const Tensor work = torch::empty({3 * n + 1}, src.options());
+  int* w = work.data_ptr<int>();
+  sp::pages_pairs(src.data_ptr<int>(), dst.data_ptr<int>(), (int)n, (int)pages, (int)block_size, w + 1, w, err_word(),
+                  stream());
+  sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, std::min(n, pages), nullptr, 0, nullptr, 0,
+                 num_sms(), stream());
+  return 2;
+}
+
+int64_t fork_pages(const Tensor& table, const Tensor& lens, const Tensor& parents, const Tensor& refs,
+                   int64_t block_size, const Tensor& new_table, const Tensor& new_lens) {
+  check_page_table(table, refs, "fork_pages");
+  check_page_table(new_table, refs, "fork_pages");
+  CHECK_I32(lens); CHECK_CONTIG(lens); CHECK_I32(parents); CHECK_CONTIG(parents); CHECK_I32(new_lens);
+  TORCH_CHECK(block_size >= 1 && block_size <= INT_MAX, "fork_pages: block_size");
+  TORCH_CHECK(lens.dim() == 1 && lens.numel() == table.size(0), "fork_pages: one length per block_table row");
+  TORCH_CHECK(parents.dim() == 1 && new_table.size(0) == parents.numel() && new_table.size(1) == table.size(1) &&
+              new_lens.numel() == parents.numel(), "fork_pages: one parent per new row");
+  CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, parents); CHECK_ON(table, refs);
+  CHECK_ON(table, new_table); CHECK_ON(table, new_lens);
+  const c10::cuda::CUDAGuard guard(table.device());
+  if (table.size(0) + parents.numel() == 0) return 0;
+  sp::pages_fork(table.data_ptr<int>(), (int)table.size(0), (int)table.size(1), lens.data_ptr<int>(),
+                 parents.data_ptr<int>(), (int)parents.numel(), refs.data_ptr<int>(), (int)refs.numel(),
+                 (int)block_size, new_table.data_ptr<int>(), new_lens.data_ptr<int>(), stream());
+  return 1;
+}
+
+int64_t reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& data,
+                      const c10::optional<Tensor>& scales, const c10::optional<Tensor>& row_tokens, int64_t tokens,
+                      int64_t block_size, const Tensor& short_by) {
+  check_page_table(table, refs, "reserve_pages");
+  const int64_t rows = table.size(0);
+  CHECK_I32(lens); CHECK_CONTIG(lens); CHECK_I32(short_by); CHECK_CONTIG(short_by);
+  TORCH_CHECK(lens.dim() == 1 && lens.numel() == rows && short_by.numel() == rows,
+              "reserve_pages: one length per block_table row");
+  TORCH_CHECK(rows <= sp::kPagesMaxRows, "reserve_pages: at most " + std::to_string(sp::kPagesMaxRows) + " rows");
+  TORCH_CHECK(tokens >= 0 && tokens <= INT_MAX, "reserve_pages: tokens must not be negative");
+  sp::PagePlane a, b;
+  const int64_t pages = page_planes(data, scales, block_size, &a, &b, "reserve_pages");
+  TORCH_CHECK(refs.numel() <= pages, "reserve_pages: refs counts more pages than the cache has");
+  if (row_tokens.has_value()) {
+    CHECK_I32(*row_tokens); CHECK_CONTIG(*row_tokens);
+    TORCH_CHECK(row_tokens->dim() == 1 && row_tokens->numel() == rows, "reserve_pages: one token count per row");
+    CHECK_ON(table, *row_tokens);
+  }
+  CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, refs); CHECK_ON(table, data); CHECK_ON(table, short_by);
+  const c10::cuda::CUDAGuard guard(table.device());
+  if (rows == 0) return 0;
+  const Tensor work = torch::empty({1 + 3 * rows + refs.numel()}, table.options());
+  int* w = work.data_ptr<int>();
+  sp::pages_reserve(table.data_ptr<int>(), (int)rows, (int)table.size(1), lens.data_ptr<int>(),
+                    row_tokens.has_value() ? row_tokens->data_ptr<int>() : nullptr, (int)tokens,
+                    refs.data_ptr<int>(), (int)refs.numel(), (int)block_size, w + 1 + 3 * rows, w + 1, w,
+                    short_by.data_ptr<int>(), stream());
+  if (data.numel() == 0) return 1;
+  sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, std::min<int64_t>(rows, refs.numel()), nullptr, 0,
+                 nullptr, 0, num_sms(), stream());
+  return 2;
+}
+
+int64_t free_pages(const Tensor& table, const Tensor& refs, const c10::optional<Tensor>& rows) {
+  check_page_table(table, refs, "free_pages");
+  if (rows.has_value()) {
+    CHECK_I32(*rows); CHECK_CONTIG(*rows);
+    TORCH_CHECK(rows->dim() == 1 && rows->numel() <= INT_MAX, "free_pages: rows must be [n]");
+    CHECK_ON(table, *rows);
+  }
+  CHECK_CUDA(table); CHECK_ON(table, refs);
+  const c10::cuda::CUDAGuard guard(table.device());
+  if (table.size(0) == 0 || (rows.has_value() && rows->numel() == 0)) return 0;
+  sp::pages_free(table.data_ptr<int>(), (int)table.size(0), (int)table.size(1), refs.data_ptr<int>(),
+                 (int)refs.numel(), rows.has_value() ? rows->data_ptr<int>() : nullptr,
+                 rows.has_value() ? (int)rows->numel() : 0, stream());
+  return 1;
+}
+
+int64_t compact_pages(const Tensor& table, const Tensor& refs, const Tensor& data, const c10::optional<Tensor>& scales,
+                      int64_t block_size, const Tensor& page_map, const Tensor& live) {
+  check_page_table(table, refs, "compact_pages");
+  sp::PagePlane a, b;
+  const int64_t pages = page_planes(data, scales, block_size, &a, &b, "compact_pages");
+  TORCH_CHECK(refs.numel() <= pages, "compact_pages: refs counts more pages than the cache has");
+  CHECK_I32(page_map); CHECK_CONTIG(page_map); CHECK_I32(live);
+  TORCH_CHECK(page_map.numel() == refs.numel() && live.numel() == 1, "compact_pages: output shapes");
+  CHECK_CUDA(table); CHECK_ON(table, refs); CHECK_ON(table, data); CHECK_ON(table, page_map); CHECK_ON(table, live);
+  const c10::cuda::CUDAGuard guard(table.device());
+  const int64_t n = refs.numel();
+  const Tensor work = torch::empty({1 + 4 * n}, table.options());
+  int* w = work.data_ptr<int>();
+  sp::pages_compact(refs.data_ptr<int>(), (int)n, (int)block_size, page_map.data_ptr<int>(), live.data_ptr<int>(),
+                    w + 1, w + 1 + 3 * n, w, stream());
+  sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, n / 2, table.data_ptr<int>(), table.numel(),
+                 page_map.data_ptr<int>(), (int)n, num_sms(), stream());
+  return 2;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1126,6 +1306,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("top2_rows", &top2_rows);
   m.def("phase_mark", &phase_mark);
   m.def("kv_blocks_copy", &kv_blocks_copy);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("copy_pages", &copy_pages);
+  m.def("fork_pages", &fork_pages);
+  m.def("reserve_pages", &reserve_pages);
+  m.def("free_pages", &free_pages);
+  m.def("compact_pages", &compact_pages);
+  m.attr("LOGPROBS_MAX_TOP") = sp::kLogprobsMaxTop;
+  m.attr("PAGES_MAX_ROWS") = sp::kPagesMaxRows;
   m.def("slab_add_rmsnorm", &slab_add_rmsnorm);
   m.def("mla_decode_prep", &mla_decode_prep);
   m.def("combine_add_rmsnorm", &combine_add_rmsnorm);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -49,6 +50,14 @@ __all__ = [
     "slab_add_rmsnorm",
     "mla_decode_prep",
     "combine_add_rmsnorm",
+    "TokenLogprobs",
+    "token_logprobs",
+    "linear_logprobs",
+    "copy_pages",
+    "fork_pages",
+    "reserve_pages",
+    "free_pages",
+    "compact_pages",
     "status_word",
     "clear_status",
     "SWAP_AB_MAX_TOKENS",
@@ -589,6 +598,122 @@ def sample_tokens(logits, temperature=0.0, seed=0, offset=0, out_ids=None, out_l
     kernels().sample_tokens(logits, float(temperature), int(seed), int(offset), out_ids, out_logit, row_temp, row_key)
     _count(1)
     return out_ids
+
+
+class TokenLogprobs(NamedTuple):
+    """Log probabilities of logits rows (natural logarithms, fp32)."""
+
+    logprobs: torch.Tensor      # of the given tokens, the shape of ids
+    entropy: torch.Tensor       # [T] of each row's distribution
+    top_logprobs: torch.Tensor  # [T, top_k] of the most probable tokens
+    top_ids: torch.Tensor       # [T, top_k] int32
+
+
+def token_logprobs(logits, ids, top_k=0) -> TokenLogprobs:
+    """Log probabilities of given tokens, the rows' entropy and their ``top_k`` most
+    probable tokens.
+
+    ``logits`` [T, V] bf16, fp16 or fp32 with unit column stride (any row stride, also a
+    view of padded rows); ``ids`` int32 [T] or [T, n]. An id of -1 asks for nothing and
+    gets 0; any other id outside [0, V) gets NaN. ``top_k`` is at most min(32, V); the
+    alternatives come by falling logit, equal ones by rising id. Tokens of probability
+    zero (logit -inf) are no alternatives: their places hold id -1 and -inf. A row that is
+    all -inf has log probability -inf and entropy 0; a row with NaN or +inf has NaN
+    everywhere and ids -1. Graph-capturable; uses no workspace."""
+    T, k = logits.shape[0], int(top_k)
+    if k < 0:
+        raise ValueError("token_logprobs: top_k must not be negative")
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    out = TokenLogprobs(torch.empty(ids.shape, **f32), torch.empty(T, **f32), torch.empty(T, k, **f32),
+                        torch.empty(T, k, dtype=torch.int32, device=logits.device))
+    kernels().token_logprobs(logits, ids, *out)
+    _count(1 if T else 0)
+    return out
+
+
+def linear_logprobs(x, w, ids):
+    """Log probabilities of given tokens and entropy of softmax(x @ w.T), without keeping
+    the logits: prompt scoring straight from hidden states and the LM head.
+
+    ``x`` [T, K] (row-major view) and ``w`` [V, K] bf16, K a multiple of 8; ``ids`` int32
+    [T] (-1: nothing asked, 0). Logits are the fp32 accumulators, not rounded to bf16.
+    Returns (logprobs [T], entropy [T]) fp32."""
+    T, V = x.shape[0], w.shape[0]
+    if ids.shape != (T,):
+        raise ValueError("linear_logprobs: ids must be [T], one per row of x")
+    f32 = dict(dtype=torch.float32, device=x.device)
+    lp, entropy = torch.empty(T, **f32), torch.empty(T, **f32)
+    rows = max(1, min(T, (1 << 28) // max(V, 1)))
+    buf = torch.empty(rows, -(-V // 4) * 4, **f32)
+    for r in range(0, T, rows):
+        n = min(rows, T - r)
+        logits = linear(x[r:r + n], w, out=buf[:n, :V], splits=1)
+        part = token_logprobs(logits, ids[r:r + n])
+        lp[r:r + n] = part.logprobs
+        entropy[r:r + n] = part.entropy
+    return lp, entropy
+
+
+# ------------------------------------------------------------------ shared cache pages
+# A block table [rows, columns] int32 holds the page of every block_size tokens of a row, -1
+# where it has none; refs [pages] int32 counts the table entries that hold a page (0: free).
+def copy_pages(cache_data, src, dst, block_size=64, cache_scales=None):
+    """Pages dst[i] of the cache become copies of pages src[i], in every layer.
+
+    ``cache_data`` [layers, slots, row] (and the fp8 cache's ``cache_scales`` [layers, slots,
+    n]), rows of whole 4-byte words; ``src`` / ``dst`` int32 [n], -1 skips a pair. A page may
+    be the source of many pairs; one that is the destination of two pairs, or of one pair and
+    the source of another, or that lies outside the cache, refuses the whole call: nothing
+    is copied and the status word is set."""
+    _count(kernels().copy_pages(cache_data, cache_scales, src, dst, int(block_size)))
+
+
+def fork_pages(block_table, lens, parents, refs, block_size=64):
+    """New rows that continue old ones: (block_table [n, columns], lens [n]).
+
+    New row i continues row parents[i] (-1, or any id that is no row: an empty row) with the
+    pages of its lens[parents[i]] tokens, which the rows then share. The old rows, all of
+    them, are given up: refs changes by what the new rows hold less what the old ones held.
+    No page is copied; ``reserve_pages`` makes a shared last page private before it is
+    written."""
+    n = parents.shape[0]
+    table = torch.empty(n, block_table.shape[1], dtype=torch.int32, device=block_table.device)
+    new_lens = torch.empty(n, dtype=torch.int32, device=block_table.device)
+    _count(kernels().fork_pages(block_table, lens, parents, refs, int(block_size), table, new_lens))
+    return table, new_lens
+
+
+def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, cache_scales=None):
+    """Room for ``tokens`` more tokens in every row, in place: missing pages behind lens[b]
+    are the lowest free ones, and a partly filled last page that other rows hold too is
+    replaced by a private copy of the row's tokens in it (every layer of the cache).
+
+    ``tokens``: a number (rows with lens[b] <= 0 are idle and get nothing) or int32 [rows].
+    Rows are served in order, each wholly or not at all; returns int32 [rows], the pages that
+    a row lacks (0: it may be written). The table's width bounds a row. At most
+    PAGES_MAX_ROWS rows."""
+    short = torch.empty(block_table.shape[0], dtype=torch.int32, device=block_table.device)
+    per_row = tokens if isinstance(tokens, torch.Tensor) else None
+    _count(kernels().reserve_pages(block_table, lens, refs, cache_data, cache_scales, per_row,
+                                   0 if per_row is not None else int(tokens), int(block_size), short))
+    return short
+
+
+def free_pages(block_table, refs, rows=None):
+    """The given rows (int32 [n], None: all) give their pages back: refs falls and their
+    entries become -1. Ids that are no row are skipped, a row that is named twice is freed once."""
+    _count(kernels().free_pages(block_table, refs, rows))
+
+
+def compact_pages(block_table, refs, cache_data, block_size=64, cache_scales=None):
+    """Moves the live pages (refs > 0) to the front of the cache, in place: with L of them,
+    the j-th live page at or behind L moves to the j-th free page before L, in every layer;
+    block_table and refs follow. Returns (page_map [pages] int32: each page's new place, -1
+    for a free one, for whatever else holds pages; L as int32 [1])."""
+    page_map = torch.empty(refs.shape[0], dtype=torch.int32, device=refs.device)
+    live = torch.empty(1, dtype=torch.int32, device=refs.device)
+    _count(kernels().compact_pages(block_table, refs, cache_data, cache_scales, int(block_size), page_map, live))
+    return page_map, live
 
 
 def gather_prev_tokens(ids, prev, n):
