@@ -327,7 +327,7 @@ void kv_blocks_copy(void* cache, long long layer_stride, const int* blocks, int 
 // dtype 0 bf16, 1 fp16, 2 fp32; ids [rows, given].
 constexpr int kLogprobsMaxTop = 32;
 void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,
-                    float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s);
+                    int num_sms, float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s);
 // Pages of a paged cache shared by several sequences (kv_pages.cu). A plane is [layers][pages][page
 // bytes] with `layer_stride` bytes between layers (base null: no plane). `work` holds (source,
 // destination, tokens) records, `copies` their number.

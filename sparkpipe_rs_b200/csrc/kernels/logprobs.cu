@@ -5,14 +5,31 @@
 //   log p_i = (x_i - m) - ln S,   entropy = ln S - E / S.
 // m, S and E come from one pass: a running maximum, and sums that are rescaled when it
 // grows. (x_i - m) is formed before ln S is taken off, so rows of the type's lowest value
-// keep their probabilities. Sums are fp32 per thread and joined in fp64.
+// keep their probabilities. Terms are added up per batch of a thread, the batches with
+// their rounding errors kept (two fp32 words), the threads in fp64: a row with one sure
+// token keeps what the others weigh, and ln S is log1p of it.
 //
 // Rows without a distribution: all -inf (a mask that leaves nothing) has log p = -inf,
 // entropy 0 and no alternatives; a row with NaN or +inf gives NaN and no alternatives.
 // Alternatives are ordered by logit, then by lower id; -inf logits are none (id -1, -inf).
+//
+// What bounds it: one read of the logits. At 8,192 rows x 102,400 bf16 an SM takes in 11
+// logits per clock, which leaves room for about eleven instructions and one exponential
+// (16 per clock) for each, so the loop works on packed pairs. The alternatives cost one
+// comparison per batch: while it streams, a thread notes the maximum of each batch of 16
+// or 32 logits in shared memory. Of the 64 maxima of four threads each, the k-th largest
+// is a floor under the row's k-th largest logit; afterwards only batches whose maximum
+// reaches it are read again (about k of them), and the logits at or above the floor are
+// ranked by counting. Should ties leave more of them than the list holds, k rounds of
+// the CTA's maximum pick them one by one.
+//
+// Few rows are split over the CTAs of a thread-block cluster, which join their sums and
+// lists through distributed shared memory: one launch, no workspace, nothing that two
+// streams or graphs could share.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <stdexcept>
 
 #include "common.cuh"
@@ -24,142 +41,684 @@ namespace sp {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+// 64 registers: with 48 the loop spills, with 80 fewer warps hide the exponentials (8,192 rows x
+// 102,400 without alternatives: 296 us, against 314 at five CTAs and 322 at three)
+constexpr int kCtasPerSm = 4;
+constexpr int kBatch = 4;         // 16-byte vectors of a batch, in flight together
+constexpr int kSlots = 16;        // recorded batch maxima of a thread (several batches each in longer rows)
+constexpr int kGroups = 64;
+constexpr int kGroupThreads = kThreads / kGroups;
+constexpr int kList = 1024;       // logits at or above the floor
+constexpr int kHot = 512;         // (thread, slot) entries whose batches reach it
+constexpr int kMaxCluster = 8;
+constexpr int kNone = 0x7fffffff;
 
-SP_DEVI float to_f32(float v) { return v; }
-SP_DEVI float to_f32(__half v) { return __half2float(v); }
-SP_DEVI float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+using u64t = unsigned long long;
 
-struct Stat {
-  float m;   // running maximum
-  float s;   // sum 2^((x - m) log2 e)
-  float e;   // sum of the same terms times (x - m) log2 e
+// Packed fp32 pairs (one instruction for two).
+SP_DEVI u64t pack2(float a, float b) {
+  u64t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+SP_DEVI void unpack2(u64t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+SP_DEVI u64t add2(u64t a, u64t b) {
+  u64t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SP_DEVI u64t mul2(u64t a, u64t b) {
+  u64t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SP_DEVI u64t fma2(u64t a, u64t b, u64t c) {
+  u64t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+SP_DEVI unsigned max_nan_bf16x2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+SP_DEVI unsigned max_nan_f16x2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// max that keeps NaN
+SP_DEVI float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16 bytes of logits: their values, and the maximum (NaN dropped) of two such vectors.
+template <typename T>
+struct Logits;
+template <>
+struct Logits<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static constexpr unsigned kNegInf = 0xff80ff80u;
+  // logits below `kLow` (-1e30) weigh nothing beside a maximum within (kMin, kMax)
+  static constexpr float kMin = -1e29f, kMax = 1e29f;
+  static SP_DEVI unsigned raise(unsigned w) { return max_nan_bf16x2(w, 0xf149f149u); }
+  static SP_DEVI float value(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static SP_DEVI void pair(unsigned w, float& a, float& b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+  }
+  static SP_DEVI unsigned max2(unsigned a, unsigned b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
+};
+template <>
+struct Logits<__half> {
+  static constexpr int N = 8;
+  static constexpr unsigned kNegInf = 0xfc00fc00u;
+  static constexpr float kMin = -60000.f, kMax = 65504.f * 2;  // raised to the type's lowest value, -65504
+  static SP_DEVI unsigned raise(unsigned w) { return max_nan_f16x2(w, 0xfbfffbffu); }
+  static SP_DEVI float value(__half v) { return __half2float(v); }
+  static SP_DEVI void pair(unsigned w, float& a, float& b) {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
+    a = f.x;
+    b = f.y;
+  }
+  static SP_DEVI unsigned max2(unsigned a, unsigned b) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
+};
+template <>
+struct Logits<float> {
+  static constexpr int N = 4;
+  static constexpr unsigned kNegInf = 0xff800000u;
+  static constexpr float kMin = -1e29f, kMax = 1e29f;
+  static SP_DEVI unsigned raise(unsigned w) { return __float_as_uint(max_nan(__uint_as_float(w), -1e30f)); }
+  static SP_DEVI float value(float v) { return v; }
+  static SP_DEVI void pair(unsigned, float&, float&) {}
+  static SP_DEVI unsigned max2(unsigned a, unsigned b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
 };
 
-// Joins two partial sums; a part without terms has m = -inf and s = e = 0.
-SP_DEVI void join(float& m, double& s, double& e, float m2, double s2, double e2) {
-  const float top = fmaxf(m, m2);
-  if (top == -INFINITY) {  // neither part has a term (NaN sums pass through)
-    s += s2;
-    e += e2;
-    return;
+// Values 2 j and 2 j + 1 of a vector.
+template <typename T>
+SP_DEVI void values2(const uint4& v, int j, float& a, float& b) {
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+  if (sizeof(T) == 4) {
+    a = __uint_as_float(w[2 * j]);
+    b = __uint_as_float(w[2 * j + 1]);
+  } else {
+    Logits<T>::pair(w[j], a, b);
   }
-  const float d1 = m == -INFINITY ? 0.f : (m - top) * kLog2e, d2 = m2 == -INFINITY ? 0.f : (m2 - top) * kLog2e;
-  const double w1 = exp2f(fmaxf(d1, -300.f)), w2 = exp2f(fmaxf(d2, -300.f));
-  // terms of a part at distance d from the new maximum: t' = t + d
-  const double t1 = fmaxf(d1, -300.f), t2 = fmaxf(d2, -300.f);
-  e = w1 * (e + s * t1) + w2 * (e2 + s2 * t2);
-  s = w1 * s + w2 * s2;
-  m = top;
+}
+
+template <typename T>
+SP_DEVI float batch_max(const uint4 (&v)[kBatch]) {
+  using L = Logits<T>;
+  unsigned m = L::max2(L::max2(v[0].x, v[0].y), L::max2(v[0].z, v[0].w));
+#pragma unroll
+  for (int i = 1; i < kBatch; ++i) m = L::max2(m, L::max2(L::max2(v[i].x, v[i].y), L::max2(v[i].z, v[i].w)));
+  if (sizeof(T) == 4) return __uint_as_float(m);
+  float a, b;
+  L::pair(m, a, b);
+  return fmaxf(a, b);
+}
+
+// Running sums of a thread: terms 2^u, u = (x - m) log2 e, in hi + lo, and terms 2^u u in e.
+struct Sums {
+  float m = -INFINITY, hi = 0.f, lo = 0.f, e = 0.f;
+
+  SP_DEVI void raise(float top) {  // a larger maximum
+    if (top > m) {
+      const float d = fmaxf((m - top) * kLog2e, -300.f);  // m = -inf: the sums are 0
+      const float w = fast_exp2(d);
+      e = w * fmaf(hi, d, e);
+      hi *= w;
+      lo *= w;
+      m = top;
+    }
+  }
+  SP_DEVI float shift() const { return m == -INFINITY ? 0.f : -m; }  // only -inf so far: u = -inf
+  SP_DEVI void add(float s, float f) {
+    const float t = hi + s, z = t - hi;
+    lo += (hi - (t - z)) + (s - z);
+    hi = t;
+    e += f;
+  }
+};
+
+// Adds the terms of two logits. CLAMP bounds u below, so that 0 * u stays 0 for -inf (and for
+// differences past fp32's range).
+template <bool CLAMP>
+SP_DEVI void term2(float a, float b, u64t shift, u64t& s, u64t& e) {
+  u64t u = mul2(add2(pack2(a, b), shift), pack2(kLog2e, kLog2e));
+  float u0, u1;
+  unpack2(u, u0, u1);
+  if (CLAMP) {
+    u0 = max_nan(u0, -200.f);
+    u1 = max_nan(u1, -200.f);
+    u = pack2(u0, u1);
+  }
+  const u64t p = pack2(fast_exp2(u0), fast_exp2(u1));
+  s = add2(s, p);
+  e = fma2(p, u, e);
+}
+
+// The sums of a batch's terms. Beside a maximum of ordinary size (CLAMP false) very small
+// logits are raised, two in one instruction, so that -inf needs no care further on.
+template <typename T, bool CLAMP>
+SP_DEVI void batch_terms(const uint4 (&v)[kBatch], float shift, float& s, float& e) {
+  using L = Logits<T>;
+  const u64t sh = pack2(shift, shift);
+  u64t s0 = 0, s1 = 0, e0 = 0, e1 = 0;
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    uint4 r = v[i];
+    if (!CLAMP) r = make_uint4(L::raise(r.x), L::raise(r.y), L::raise(r.z), L::raise(r.w));
+#pragma unroll
+    for (int j = 0; j < L::N / 2; j += 2) {
+      float f0, f1, f2, f3;
+      values2<T>(r, j, f0, f1);
+      values2<T>(r, j + 1, f2, f3);
+      term2<CLAMP>(f0, f1, sh, s0, e0);
+      term2<CLAMP>(f2, f3, sh, s1, e1);
+    }
+  }
+  float p, q;
+  unpack2(add2(s0, s1), p, q);
+  s = p + q;
+  unpack2(add2(e0, e1), p, q);
+  e = p + q;
+}
+
+struct Batch {
+  uint4 v[kBatch];
+};
+// Out of line: rows of nothing but masked logits so far, huge logits, NaN.
+template <typename T>
+__device__ __noinline__ float2 rare_terms(Batch b, float shift) {
+  float2 r;
+  batch_terms<T, true>(b.v, shift, r.x, r.y);
+  return r;
 }
 
 // (v, i) ranks before (w, j): larger logit, then lower id
 SP_DEVI bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
-}  // namespace
-
+// This CTA's part of a row: single logits before the first 16-byte boundary and behind the
+// last whole vector (at most one each per thread), vectors in between.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V,
-                                                                  const int* __restrict__ ids, int given, int k,
-                                                                  float* __restrict__ lp, float* __restrict__ entropy,
-                                                                  float* __restrict__ top_lp, int* __restrict__ top_id) {
-  griddep_wait();
-  griddep_launch();
-  const long long row = blockIdx.x;
-  const T* x = logits + row * ld;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  Stat a = {-INFINITY, 0.f, 0.f};
-  for (int c = threadIdx.x; c < V; c += kThreads) {
-    const float v = to_f32(x[c]);
-    const float top = fmaxf(a.m, v);
-    if (top > a.m) {
-      const float d = a.m == -INFINITY ? 0.f : fmaxf((a.m - top) * kLog2e, -300.f);
-      a.e = exp2f(d) * (a.e + a.s * d);
-      a.s *= exp2f(d);
-      a.m = top;
-    }
-    if (v == -INFINITY) continue;
-    const float t = v - a.m;  // NaN for NaN and +inf logits: the sums carry it
-    const float u = t < -200.f ? -200.f : t * kLog2e;
-    const float p = exp2f(u);
-    a.s += p;
-    a.e += p * u;
+struct Part {
+  const T* row;
+  const uint4* body;
+  int first;      // id of the body's first logit
+  int v0, v1;     // this CTA's vectors
+  int head, tail; // id of this thread's single logits, -1 for none
+
+  SP_DEVI Part(const T* r, int V, int rank, int parts) : row(r) {
+    constexpr int N = Logits<T>::N;
+    const int skip = int((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / (int)sizeof(T);
+    first = min(skip, V);
+    body = reinterpret_cast<const uint4*>(r + first);
+    const int nv = (V - first) / N;
+    v0 = int((long long)nv * rank / parts);
+    v1 = int((long long)nv * (rank + 1) / parts);
+    const int t = threadIdx.x;
+    head = rank == 0 && t < first ? t : -1;
+    const int behind = first + nv * N;
+    tail = rank == parts - 1 && t < V - behind ? behind + t : -1;
   }
-  float m = a.m;
-  double s = a.s, e = a.e;
+  SP_DEVI uint4 vector(int v) const {
+    if (v < v1) return __ldg(body + v);
+    constexpr unsigned n = Logits<T>::kNegInf;
+    return make_uint4(n, n, n, n);
+  }
+  SP_DEVI float single(int id) const { return id >= 0 ? Logits<T>::value(row[id]) : -INFINITY; }
+  // calls f(logit, id) for this thread's logits in batches [b0, b1) (vectors) or its single ones
+  template <typename F>
+  SP_DEVI void batches(int b0, int b1, F f) const {
+    for (int b = b0; b < b1; ++b) {
+      uint4 v[kBatch];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    join(m, s, e, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o),
-         __shfl_xor_sync(0xffffffffu, e, o));
-  __shared__ float sm[kThreads / 32];
-  __shared__ double ss[kThreads / 32], se[kThreads / 32];
-  __shared__ float bv[kThreads / 32];
-  __shared__ int bi[kThreads / 32];
-  if (lane == 0) {
-    sm[w] = m;
-    ss[w] = s;
-    se[w] = e;
-  }
-  __syncthreads();
-  m = sm[0];
-  s = ss[0];
-  e = se[0];
-  for (int i = 1; i < kThreads / 32; ++i) join(m, s, e, sm[i], ss[i], se[i]);
-  const bool bad = s != s, empty = !bad && s == 0.0;
-  const float log_s = empty ? 0.f : (s < 2.0 ? log1pf(float(s - 1.0)) : logf(float(s)));
-  const float base = empty ? 0.f : m;
-  if (threadIdx.x == 0)
-    entropy[row] = bad ? NAN : empty ? 0.f : float(log_s - e / s * 0.6931471805599453);
-  for (int j = threadIdx.x; j < given; j += kThreads) {
-    const int id = ids[row * given + j];
-    lp[row * given + j] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (to_f32(x[id]) - base) - log_s;
-  }
-  // k rounds: the best (logit, id) that ranks after the previous round's
-  float pv = INFINITY;
-  int pi = -1;
-  for (int r = 0; r < k; ++r) {
-    float best = -INFINITY;
-    int at = 0x7fffffff;
-    if (!bad && pi != 0x7fffffff)
-      for (int c = threadIdx.x; c < V; c += kThreads) {
-        const float v = to_f32(x[c]);
-        if (v != -INFINITY && before(pv, pi, v, c) && before(v, c, best, at)) { best = v; at = c; }
+      for (int i = 0; i < kBatch; ++i) v[i] = vector(v0 + (b * kBatch + i) * kThreads + threadIdx.x);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int at = first + (v0 + (b * kBatch + i) * kThreads + (int)threadIdx.x) * Logits<T>::N;
+#pragma unroll
+        for (int j = 0; j < Logits<T>::N / 2; ++j) {
+          float x, y;
+          values2<T>(v[i], j, x, y);
+          f(x, at + 2 * j);
+          f(y, at + 2 * j + 1);
+        }
       }
+    }
+  }
+  template <typename F>
+  SP_DEVI void singles(F f) const {
+    f(single(head), head);
+    f(single(tail), tail);
+  }
+};
+
+struct Stat {
+  float m;
+  double s, e;
+};
+
+struct Shared {
+  float slot[kSlots][kThreads];
+  float group[kGroups];            // maxima of four threads' logits each (of the whole cluster)
+  Stat stat[kMaxCluster * kWarps]; // the cluster's warps (first CTA)
+  float floor;
+  float base, log_s;               // the row's maximum (0 for an empty row) and ln S
+  int bad;
+  int hot_n, n;
+  int hot[kHot];                   // (thread, slot) whose batches reach the floor
+  float v[kList];                  // logits at or above the floor (first CTA)
+  int id[kList];
+};
+
+// Shared memory of the cluster's CTA q (q < 0: this CTA's own, without a cluster).
+SP_DEVI void st_f32(float* p, float v, int q) {
+  if (q < 0) *p = v;
+  else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), q)), "f"(v) : "memory");
+}
+SP_DEVI void st_f64(double* p, double v, int q) {
+  if (q < 0) *p = v;
+  else asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), q)), "d"(v) : "memory");
+}
+SP_DEVI void st_s32(int* p, int v, int q) {
+  if (q < 0) *p = v;
+  else asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), q)), "r"(v) : "memory");
+}
+SP_DEVI int add_s32(int* p, int v, int q) {
+  if (q < 0) return atomicAdd(p, v);
+  int r;
+  asm volatile("atom.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(r) : "r"(mapa_shared(smem_u32(p), q)), "r"(v) : "memory");
+  return r;
+}
+
+// Joins the warps' sums; every lane of the calling warp gets the row's (m, S, E).
+SP_DEVI void join_stats(const Shared& sh, int n, float& m, double& s, double& e) {
+  const int lane = threadIdx.x & 31;
+  m = -INFINITY;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, sh.stat[i].m);
+  m = warp_max(m);
+  s = e = 0.0;
+  for (int i = lane; i < n; i += 32) {
+    const Stat t = sh.stat[i];
+    const float d = t.m == -INFINITY ? 0.f : fmaxf((t.m - m) * kLog2e, -300.f);
+    const double f = fast_exp2(d);
+    s += f * t.s;
+    e += f * (t.e + t.s * d);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    e += __shfl_xor_sync(0xffffffffu, e, o);
+  }
+}
+
+// More logits reach the floor than the list holds: each thread offers its best one not
+// yet taken, the CTA takes the best of these, k times.
+template <typename T>
+__device__ __noinline__ void pick_rounds(const Part<T>& part, int nb, int k, Shared& sh) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  float pv = INFINITY, best = -INFINITY;
+  int pi = -1, at = kNone;
+  bool scan = true;
+  for (int r = 0; r < k; ++r) {
+    if (scan) {
+      best = -INFINITY;
+      at = kNone;
+      auto see = [&](float v, int i) {
+        if (v != -INFINITY && i >= 0 && before(pv, pi, v, i) && before(v, i, best, at)) { best = v; at = i; }
+      };
+      part.batches(0, nb, see);
+      part.singles(see);
+    }
+    float bv = best;
+    int bi = at;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-      if (before(ov, oi, best, at)) { best = ov; at = oi; }
+      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+      if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
     }
     __syncthreads();
     if (lane == 0) {
-      bv[w] = best;
-      bi[w] = at;
+      sh.v[w] = bv;
+      sh.id[w] = bi;
     }
     __syncthreads();
-    best = bv[0];
-    at = bi[0];
-    for (int i = 1; i < kThreads / 32; ++i)
-      if (before(bv[i], bi[i], best, at)) { best = bv[i]; at = bi[i]; }
-    pv = best;
-    pi = at;
+    for (int i = 0; i < kWarps; ++i)
+      if (before(sh.v[i], sh.id[i], bv, bi)) { bv = sh.v[i]; bi = sh.id[i]; }
     if (threadIdx.x == 0) {
-      const bool none = at == 0x7fffffff;
-      top_id[row * k + r] = none ? -1 : at;
-      top_lp[row * k + r] = bad ? NAN : none ? -INFINITY : (best - base) - log_s;
+      sh.v[kWarps + r] = bv;
+      sh.id[kWarps + r] = bi;
+      if (bi != kNone) sh.n = r + 1;
+    }
+    pv = bv;
+    pi = bi;
+    scan = bi != kNone && bi == at;  // this thread's offer was taken
+    if (bi == kNone) break;
+  }
+  __syncthreads();
+}
+
+}  // namespace
+
+// One row per cluster of `parts` CTAs (1: no cluster).
+template <typename T, bool TOP, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const int* __restrict__ ids, int given,
+                          int k, int parts, float* __restrict__ lp, float* __restrict__ entropy,
+                          float* __restrict__ top_lp, int* __restrict__ top_id) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int rank = CLUSTER ? (int)cluster_ctarank() : 0;
+  const long long row = CLUSTER ? blockIdx.x / parts : blockIdx.x;
+  if (CLUSTER) cluster_sync();  // all its CTAs have started: they will write one another's shared memory
+  griddep_wait();
+  griddep_launch();
+  const T* x = logits + row * ld;
+  const Part<T> part(x, V, rank, CLUSTER ? parts : 1);
+  // the first given tokens' logits, on their way while the row streams
+  int id = -1;
+  float xid = 0.f;
+  if (rank == 0 && (int)threadIdx.x < given) {
+    id = ids[row * given + threadIdx.x];
+    if (id >= 0 && id < V) xid = Logits<T>::value(x[id]);
+  }
+  const int nb = (part.v1 - part.v0 + kBatch * kThreads - 1) / (kBatch * kThreads);
+  const int per_slot = (nb + kSlots - 1) / kSlots;
+
+  Sums a;
+  float slot_max = -INFINITY;
+  int slot = 0, left = per_slot;
+  auto take = [&](uint4 (&v)[kBatch]) {
+    const float top = batch_max<T>(v);
+    a.raise(top);
+    float bs, be;
+    if (a.m > Logits<T>::kMin && a.m < Logits<T>::kMax) {
+      batch_terms<T, false>(v, -a.m, bs, be);
+    } else {
+      Batch copy;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) copy.v[i] = v[i];
+      const float2 r = rare_terms<T>(copy, a.shift());
+      bs = r.x;
+      be = r.y;
+    }
+    a.add(bs, be);
+    if (TOP && per_slot == 1) {
+      sh.slot[slot++][threadIdx.x] = top;
+    } else if (TOP) {
+      slot_max = fmaxf(slot_max, top);
+      if (--left == 0) {
+        sh.slot[slot++][threadIdx.x] = slot_max;
+        slot_max = -INFINITY;
+        left = per_slot;
+      }
+    }
+  };
+  const int whole = (part.v1 - part.v0) / (kBatch * kThreads);
+  const uint4* src = part.body + part.v0 + threadIdx.x;
+#pragma unroll 1
+  for (int b = 0; b < whole; ++b) {
+    uint4 v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) v[i] = __ldg(src + i * kThreads);
+    src += kBatch * kThreads;
+    take(v);
+  }
+  if (whole < nb) {
+    uint4 v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) v[i] = part.vector(part.v0 + (whole * kBatch + i) * kThreads + threadIdx.x);
+    take(v);
+  }
+  if (TOP && per_slot > 1 && left != per_slot) sh.slot[slot++][threadIdx.x] = slot_max;
+  const float one = part.single(part.head), two = part.single(part.tail);
+  if (part.head >= 0 || part.tail >= 0) {
+    const float top = fmaxf(one, two);
+    a.raise(top);
+    const float shift = a.shift();
+    u64t s0 = 0, e0 = 0;
+    term2<true>(one, two, pack2(shift, shift), s0, e0);
+    float p, q, f, g;
+    unpack2(s0, p, q);
+    unpack2(e0, f, g);
+    a.add(p + q, f + g);
+  }
+
+  // the warps' sums, to the cluster's first CTA; 64 group maxima, to all its CTAs
+  const int first = CLUSTER ? 0 : -1;
+  float m = a.m;
+  if (TOP && !CLUSTER) {
+#pragma unroll
+    for (int o = 1; o < kGroupThreads; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane % kGroupThreads == 0) sh.group[threadIdx.x / kGroupThreads] = m;
+  }
+  if (TOP && CLUSTER) {
+    const int wide = kGroupThreads * parts;  // threads of a group, at most a warp
+    for (int o = 1; o < wide; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane % wide == 0)
+      for (int q = 0; q < parts; ++q) st_f32(&sh.group[(rank * kThreads + threadIdx.x) / wide], m, q);
+  }
+  m = warp_max(m);
+  {
+    const float d = a.m == -INFINITY ? 0.f : fmaxf((a.m - m) * kLog2e, -300.f);
+    const float f = fast_exp2(d);
+    double s = double(a.hi * f) + double(a.lo * f), e = double(f * fmaf(a.hi, d, a.e));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      e += __shfl_xor_sync(0xffffffffu, e, o);
+    }
+    if (lane == 0) {
+      Stat* t = &sh.stat[rank * kWarps + w];
+      st_f32(&t->m, m, first);
+      st_f64(&t->s, s, first);
+      st_f64(&t->e, e, first);
+    }
+  }
+  if (TOP && threadIdx.x == 0) sh.n = sh.hot_n = 0;
+  if (CLUSTER) cluster_sync();
+  else __syncthreads();
+
+  // the join by the last warp of the first CTA, the floor by the first warp of each
+  if (rank == 0 && w == kWarps - 1) {
+    double s, e;
+    join_stats(sh, (CLUSTER ? parts : 1) * kWarps, m, s, e);
+    if (lane == 0) {
+      const bool bad = s != s, empty = !bad && s == 0.0;
+      const float log_s = empty ? 0.f : s < 2.0 ? log1pf(float(s - 1.0)) : logf(float(s));
+      sh.bad = bad;
+      sh.base = empty ? 0.f : m;
+      sh.log_s = log_s;
+      entropy[row] = bad ? NAN : empty ? 0.f : float(log_s - e / s * kLn2);
+    }
+  }
+  int n = 0;
+  if (TOP) {
+    if (w == 0) {
+      // the largest group maximum that k of the 64 reach
+      const float g0 = sh.group[lane], g1 = sh.group[lane + 32];
+      int r0 = 0, r1 = 0;
+#pragma unroll
+      for (int i = 0; i < kGroups; i += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(&sh.group[i]);
+        r0 += (g.x >= g0) + (g.y >= g0) + (g.z >= g0) + (g.w >= g0);
+        r1 += (g.x >= g1) + (g.y >= g1) + (g.z >= g1) + (g.w >= g1);
+      }
+      const float f = warp_max(fmaxf(r0 >= k ? g0 : -INFINITY, r1 >= k ? g1 : -INFINITY));
+      if (lane == 0) sh.floor = f;
+    }
+    __syncthreads();
+    const float floor = sh.floor;
+    auto see = [&](float v, int i) {
+      if (v >= floor && v != -INFINITY && i >= 0) {
+        const int at = add_s32(&sh.n, 1, first);
+        if (at < kList) {
+          st_f32(&sh.v[at], v, first);
+          st_s32(&sh.id[at], i, first);
+        }
+      }
+    };
+    if (a.m >= floor && a.m != -INFINITY) {
+#pragma unroll 4
+      for (int q = 0; q < slot; ++q)
+        if (sh.slot[q][threadIdx.x] >= floor) {
+          const int at = atomicAdd(&sh.hot_n, 1);
+          if (at < kHot) sh.hot[at] = q * kThreads + threadIdx.x;
+        }
+      if (fmaxf(one, two) >= floor) part.singles(see);
+    }
+    __syncthreads();
+    // one warp per entry: its batches' logits side by side, a lane each
+    const int entries = sh.hot_n;
+    if (entries > kHot) {
+      if (threadIdx.x == 0) add_s32(&sh.n, kList + 1, first);
+    } else {
+      constexpr int N = Logits<T>::N, kAhead = 4;
+      const int pieces = (per_slot * kBatch * N + 31) / 32;  // of an entry, a logit per lane
+      for (int i0 = w; i0 < entries * pieces; i0 += kAhead * kWarps) {
+        float v[kAhead];
+        int at[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {  // loads first: they come from L2 or memory
+          const int i = i0 + u * kWarps;
+          at[u] = -1;
+          v[u] = -INFINITY;
+          if (i < entries * pieces) {
+            const int entry = pieces == 1 ? i : i / pieces;
+            const int t = sh.hot[entry] % kThreads, q = sh.hot[entry] / kThreads;
+            const int j = (i - entry * pieces) * 32 + lane;
+            const int b = q * per_slot * kBatch + j / N;  // the thread's vector
+            const int vec = part.v0 + b * kThreads + t;
+            if (j < per_slot * kBatch * N && b < nb * kBatch && vec < part.v1) {
+              at[u] = part.first + vec * N + j % N;
+              v[u] = Logits<T>::value(x[at[u]]);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) see(v[u], at[u]);
+      }
+    }
+    if (CLUSTER) cluster_sync();
+    else __syncthreads();
+    if (CLUSTER && rank != 0) return;
+    n = sh.n;
+  } else {
+    if (CLUSTER && rank != 0) return;
+    __syncthreads();
+  }
+
+  const bool bad = sh.bad;
+  const float base = sh.base, log_s = sh.log_s;
+  for (int j = threadIdx.x; j < given; j += kThreads) {
+    if (j >= kThreads) {
+      id = ids[row * given + j];
+      if (id >= 0 && id < V) xid = Logits<T>::value(x[id]);
+    }
+    lp[row * given + j] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (xid - base) - log_s;
+  }
+  if (TOP) {
+    int base_at = 0;
+    if (n > kList) {
+      __syncthreads();  // every warp has read sh.n
+      const Part<T> whole(x, V, 0, 1);
+      if (threadIdx.x == 0) sh.n = 0;
+      pick_rounds(whole, (whole.v1 - whole.v0 + kBatch * kThreads - 1) / (kBatch * kThreads), k, sh);
+      n = sh.n;
+      base_at = kWarps;
+    }
+    // a logit's place is how many rank before it
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const float v = sh.v[base_at + i];
+      const int at = sh.id[base_at + i];
+      int r = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) r += before(sh.v[base_at + j], sh.id[base_at + j], v, at);
+      if (r < k) {
+        top_id[row * k + r] = bad ? -1 : at;
+        top_lp[row * k + r] = bad ? NAN : (v - base) - log_s;
+      }
+    }
+    for (int r = n + threadIdx.x; r < k; r += kThreads) {
+      top_id[row * k + r] = -1;
+      top_lp[row * k + r] = bad ? NAN : -INFINITY;
     }
   }
 }
 
-void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,
-                    float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
-  if (rows <= 0) return;
-  auto run = [&](auto* x, auto kern) {
-    launch_k(kern, dim3((unsigned)rows), dim3(kThreads), 0, s, x, ld, V, ids, given, k, lp, entropy, top_lp, top_id);
+template <typename T, bool TOP, bool CLUSTER>
+static void launch(const T* logits, long long ld, int rows, int V, const int* ids, int given, int k, int parts,
+                   float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
+  auto kern = token_logprobs_kernel<T, TOP, CLUSTER>;
+  prefer_max_smem_carveout(reinterpret_cast<const void*>(kern));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attrs[2];
+  cfg.gridDim = dim3((unsigned)(rows * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.stream = s;
+  cfg.attrs = attrs;
+  if (CLUSTER) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = parts;
+    attrs[cfg.numAttrs].val.clusterDim.y = 1;
+    attrs[cfg.numAttrs].val.clusterDim.z = 1;
+    cfg.numAttrs += 1;
+  }
+  if (pdl_enabled()) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs += 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, logits, ld, V, ids, given, k, parts, lp, entropy, top_lp,
+                                           top_id);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("token_logprobs launch failed: ") + cudaGetErrorString(e));
+}
+
+template <typename T>
+static void dispatch(const T* logits, long long ld, int rows, int V, const int* ids, int given, int k, int num_sms,
+                     float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
+  // CTAs per row: few rows are split as long as that gives each SM two CTAs at most and each
+  // CTA a whole batch. Split further, a row's join costs more than its stream gains: 64 rows x
+  // 102,400 bf16 with 20 alternatives take 16.8 us unsplit, 10.5 us in four, 11.0 us in eight;
+  // 515 rows 29.9 us unsplit, 38.0 us in two; one row 12.0 us unsplit, 6.5 us in eight.
+  const int batch = kBatch * kThreads * Logits<T>::N;
+  int parts = 1;
+  while (parts < kMaxCluster && (long long)rows * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= batch) parts *= 2;
+  auto run = [&](auto top, auto cluster) {
+    launch<T, decltype(top)::value, decltype(cluster)::value>(logits, ld, rows, V, ids, given, k, parts, lp, entropy,
+                                                              top_lp, top_id, s);
   };
-  if (dtype == 0) run(static_cast<const __nv_bfloat16*>(logits), token_logprobs_kernel<__nv_bfloat16>);
-  else if (dtype == 1) run(static_cast<const __half*>(logits), token_logprobs_kernel<__half>);
-  else run(static_cast<const float*>(logits), token_logprobs_kernel<float>);
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (k > 0) parts > 1 ? run(Yes{}, Yes{}) : run(Yes{}, No{});
+  else parts > 1 ? run(No{}, Yes{}) : run(No{}, No{});
+}
+
+void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,
+                    int num_sms, float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
+  if (rows <= 0) return;
+  auto run = [&](auto* x) { dispatch(x, ld, rows, V, ids, given, k, num_sms, lp, entropy, top_lp, top_id, s); };
+  if (dtype == 0) run(static_cast<const __nv_bfloat16*>(logits));
+  else if (dtype == 1) run(static_cast<const __half*>(logits));
+  else run(static_cast<const float*>(logits));
 }
 
 }  // namespace sp

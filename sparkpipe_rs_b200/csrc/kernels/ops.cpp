@@ -1090,32 +1090,32 @@ void ep_advance(const Tensor& epoch) {
 }
 
 // ---- log probabilities and shared cache pages
-void token_logprobs(const Tensor& logits, const Tensor& ids, const Tensor& lp, const Tensor& entropy,
-                    const Tensor& top_lp, const Tensor& top_ids) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& ids, int64_t k) {
   TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
               "token_logprobs: logits must be [T, V] with unit column stride");
   const auto st = logits.scalar_type();
   TORCH_CHECK(st == at::kBFloat16 || st == at::kHalf || st == at::kFloat,
               "token_logprobs: logits must be bf16, fp16 or fp32");
-  const int64_t T = logits.size(0), V = logits.size(1), k = top_lp.size(1);
+  const int64_t T = logits.size(0), V = logits.size(1);
   TORCH_CHECK(T == 0 || V >= 1, "token_logprobs: no columns");
-  TORCH_CHECK(T <= INT_MAX && V <= INT_MAX - 4096, "token_logprobs: too large");
+  TORCH_CHECK(T <= INT_MAX && V <= INT_MAX - 65536, "token_logprobs: too large");
   CHECK_I32(ids); CHECK_CONTIG(ids);
   TORCH_CHECK((ids.dim() == 1 || ids.dim() == 2) && ids.size(0) == T,
               "token_logprobs: ids must be [T] or [T, n], one row per logits row");
   const int64_t given = ids.dim() == 2 ? ids.size(1) : 1;
+  TORCH_CHECK(given <= INT_MAX, "token_logprobs: too many ids");
   TORCH_CHECK(k >= 0 && k <= sp::kLogprobsMaxTop && (T == 0 || k <= V),
               "token_logprobs: top_k must be between 0 and min(" + std::to_string(sp::kLogprobsMaxTop) + ", V)");
-  CHECK_F32(lp); CHECK_F32(entropy); CHECK_F32(top_lp); CHECK_I32(top_ids);
-  CHECK_CONTIG(lp); CHECK_CONTIG(entropy); CHECK_CONTIG(top_lp); CHECK_CONTIG(top_ids);
-  TORCH_CHECK(lp.numel() == ids.numel() && entropy.numel() == T && top_lp.numel() == T * k &&
-              top_ids.numel() == T * k, "token_logprobs: output shapes");
-  CHECK_CUDA(logits); CHECK_ON(logits, ids); CHECK_ON(logits, lp); CHECK_ON(logits, entropy);
-  CHECK_ON(logits, top_lp); CHECK_ON(logits, top_ids);
+  CHECK_CUDA(logits); CHECK_ON(logits, ids);
   const c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  const Tensor lp = at::empty(ids.sizes(), f32), entropy = at::empty({T}, f32), top_lp = at::empty({T, k}, f32),
+               top_ids = at::empty({T, k}, ids.options());
   sp::token_logprobs(logits.data_ptr(), st == at::kBFloat16 ? 0 : st == at::kHalf ? 1 : 2, logits.stride(0), (int)T,
-                     (int)V, ids.data_ptr<int>(), (int)given, (int)k, lp.data_ptr<float>(), entropy.data_ptr<float>(),
-                     top_lp.data_ptr<float>(), top_ids.data_ptr<int>(), stream());
+                     (int)V, ids.data_ptr<int>(), (int)given, (int)k, num_sms(), lp.data_ptr<float>(),
+                     entropy.data_ptr<float>(), top_lp.data_ptr<float>(), top_ids.data_ptr<int>(),
+                     stream());
+  return {lp, entropy, top_lp, top_ids};
 }
 
 // One plane of a paged cache [layers, slots, row]; any layer stride, rows and slots dense.

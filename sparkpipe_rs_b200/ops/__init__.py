@@ -620,14 +620,8 @@ def token_logprobs(logits, ids, top_k=0) -> TokenLogprobs:
     zero (logit -inf) are no alternatives: their places hold id -1 and -inf. A row that is
     all -inf has log probability -inf and entropy 0; a row with NaN or +inf has NaN
     everywhere and ids -1. Graph-capturable; uses no workspace."""
-    T, k = logits.shape[0], int(top_k)
-    if k < 0:
-        raise ValueError("token_logprobs: top_k must not be negative")
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    out = TokenLogprobs(torch.empty(ids.shape, **f32), torch.empty(T, **f32), torch.empty(T, k, **f32),
-                        torch.empty(T, k, dtype=torch.int32, device=logits.device))
-    kernels().token_logprobs(logits, ids, *out)
-    _count(1 if T else 0)
+    out = TokenLogprobs(*kernels().token_logprobs(logits, ids, int(top_k)))
+    _count(1 if logits.shape[0] else 0)
     return out
 
 
