@@ -328,6 +328,11 @@ void kv_blocks_copy(void* cache, long long layer_stride, const int* blocks, int 
 constexpr int kLogprobsMaxTop = 32;
 void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,
                     int num_sms, float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s);
+// The same without alternatives from x [T, K] and w [V, K] bf16, logits never in memory
+// (lm_logprobs.cu); the workspace is lm_logprobs_workspace() float4 elements.
+long long lm_logprobs_workspace(int T, int V, int num_sms);
+void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K, const int* ids,
+                 void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s);
 // Pages of a paged cache shared by several sequences (kv_pages.cu). A plane is [layers][pages][page
 // bytes] with `layer_stride` bytes between layers (base null: no plane). `work` holds (source,
 // destination, tokens) records, `copies` their number.

@@ -1,0 +1,336 @@
+// Log probabilities of given tokens and entropy straight from hidden states x [T, K] and the
+// LM head's weight w [V, K] (bf16): logits = x w^T exist only as tcgen05 accumulators, sm_100a.
+//
+// For a row of logits l: m = max l, S = sum exp(l_i - m), E = sum exp(l_i - m) (l_i - m);
+//   log p_i = (l_i - m) - ln S,   entropy = ln S - E / S.
+// A CTA walks the vocabulary tiles of its share for 128 rows, tile by tile 128 x 256 logits in
+// tensor memory, and its epilogue threads (one row of half a tile each) keep m, S, E and the
+// given token's logit running; a second kernel joins the shares of a row. The logits of an
+// 8,192-token chunk over 102,400 tokens would be 3.4 GB in fp32.
+//
+// What bounds it: the products for many rows (2 T V K operations), one read of w for few.
+//
+//  * The tensor cores add the products of a K block onto the accumulator and cut the sum off
+//    below its last bit instead of rounding: over long K the logits shrink by about 1e-6 of
+//    their size, all the same way, which shows in the entropy. So K is taken in segments of
+//    1,024, each with an accumulator of its own, and the epilogue adds the segments with
+//    rounding (K = 2,048: entropy off by 1.5e-6 with one accumulator).
+//  * Work items are (128 rows, a range of 64-token units of the vocabulary), rows fastest:
+//    the CTAs that run at the same time read the same range of w, so it comes from memory
+//    once and then from L2, and one row tile's shares are few enough to join cheaply.
+//  * Warp roles (320 threads): warp 0 TMA, warp 1 MMA and tensor memory, warps 2..9 epilogue
+//    (lane quarter = warp % 4, columns [0, 128) or [128, 256) of a tile).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "launch.h"
+#include "logprobs.cuh"
+#include "pdl.h"
+
+namespace sp {
+
+namespace {
+
+constexpr int kRows = 128;       // rows of an item
+constexpr int kCols = 256;       // logits of a tile's row
+constexpr int kUnit = 64;        // tokens of a unit: rows of one TMA box of w
+constexpr int kBlockK = 64;
+constexpr int kSegBlocks = 16;   // K blocks of a segment
+constexpr int kStages = 4;
+constexpr int kXBytes = kRows * kBlockK * 2;
+constexpr int kBoxBytes = kUnit * kBlockK * 2;
+constexpr int kStageBytes = kXBytes + kCols / kUnit * kBoxBytes;
+constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+constexpr int kHalf = 128;       // columns of an epilogue thread
+constexpr int kEpilogue = 256;   // epilogue threads
+
+struct LmParams {
+  int T, V, K;
+  int row_tiles, units, shares;  // row tiles, 64-token units, shares of a row tile
+  const int* ids;
+  float4* part;                  // [shares * 2][row_tiles * 128]: m, S, E (log2 units), the given token's logit
+  int* err;
+};
+
+SP_DEVI void share_units(const LmParams& p, int share, int& u0, int& u1) {
+  u0 = int((long long)p.units * share / p.shares);
+  u1 = int((long long)p.units * (share + 1) / p.shares);
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(64 + kEpilogue, 1)
+    lm_logprobs_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                       const LmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], kEpilogue);
+    }
+    *s_err = 0;
+    fence_mbarrier_init();
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc<2 * kCols>(tmem_slot);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch();
+  griddep_wait();
+  const uint32_t tmem = *tmem_slot;
+  const int items = p.row_tiles * p.shares;
+  const int blocks = (p.K + kBlockK - 1) / kBlockK;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t once = policy_evict_first();  // with one row tile, w only passes through L2
+      int it = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        int u0, u1;
+        share_units(p, item / p.row_tiles, u0, u1);
+        const int row = (item % p.row_tiles) * kRows;
+        for (; ok && u0 < u1; u0 += kCols / kUnit) {
+          const int n = min(kCols / kUnit, u1 - u0);
+          for (int kb = 0; kb < blocks; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutProducer)) {
+              ok = false;
+              break;
+            }
+            uint8_t* at = smem + s * kStageBytes;
+            mbar_arrive_expect_tx(&full[s], kXBytes + n * kBoxBytes);
+            tma_load_2d(at, &tmX, &full[s], kb * kBlockK, row);
+            for (int i = 0; i < n; ++i) {
+              uint8_t* box = at + kXBytes + i * kBoxBytes;
+              if (p.row_tiles == 1) tma_load_2d_hint(box, &tmW, &full[s], kb * kBlockK, (u0 + i) * kUnit, once);
+              else tma_load_2d(box, &tmW, &full[s], kb * kBlockK, (u0 + i) * kUnit);
+            }
+          }
+        }
+      }
+      // loads in flight land before the CTA gives up its memory
+      for (int j = max(0, it - kStages); j < it && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int it = 0, tc = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        int u0, u1;
+        share_units(p, item / p.row_tiles, u0, u1);
+        for (; ok && u0 < u1; u0 += kCols / kUnit) {
+          const uint32_t idesc = idesc_bf16_f32(kRows, min(kCols / kUnit, u1 - u0) * kUnit);
+          for (int kb = 0; kb < blocks; ++kb, ++it) {
+            const int buf = tc & 1;
+            if (kb % kSegBlocks == 0) {
+              if (!mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
+              tc_fence_after();
+            }
+            const int s = it % kStages;
+            if (!mbar_wait(&full[s], (it / kStages) & 1, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t at = smem_u32(smem + s * kStageBytes);
+            const uint64_t a = sdesc_kmajor_sw128(at), b = sdesc_kmajor_sw128(at + kXBytes);
+#pragma unroll
+            for (int k = 0; k < kBlockK / 16; ++k)
+              umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, (kb % kSegBlocks > 0 || k > 0) ? 1u : 0u);
+            umma_commit(&empty[s]);
+            if (kb % kSegBlocks == kSegBlocks - 1 || kb == blocks - 1) {
+              umma_commit(&tfull[buf]);
+              ++tc;
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int m = q * 32 + lane;
+    const uint32_t mine = tmem + (uint32_t(q * 32) << 16) + half * kHalf;
+    int tc = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      const int share = item / p.row_tiles;
+      int u0, u1;
+      share_units(p, share, u0, u1);
+      const int row = (item % p.row_tiles) * kRows + m;
+      const int id = row < p.T ? p.ids[row] : -1;
+      LogprobSums a;
+      float given = 0.f;
+      for (; ok && u0 < u1; u0 += kCols / kUnit) {
+        const int first = u0 * kUnit + half * kHalf;
+        // columns of this thread: up to the share's end and the vocabulary's
+        const int cols = min(kHalf, min(u1 * kUnit, p.V) - first);
+        float v[kHalf];
+        for (int kb = 0; ok && kb < blocks; kb += kSegBlocks, ++tc) {
+          const int buf = tc & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&tfull[buf], (tc >> 1) & 1, s_err, p.err, kErrWaitTimeoutEpilogue));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 32) {
+            uint32_t r0[16], r1[16];
+            tmem_ld16_issue(mine + buf * kCols + c, r0);
+            tmem_ld16_issue(mine + buf * kCols + c + 16, r1);
+            tmem_ld_wait(r0);
+            tmem_ld_wait(r1);
+            if (kb == 0) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                v[c + j] = __uint_as_float(r0[j]);
+                v[c + 16 + j] = __uint_as_float(r1[j]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                v[c + j] += __uint_as_float(r0[j]);
+                v[c + 16 + j] += __uint_as_float(r1[j]);
+              }
+            }
+          }
+          tc_fence_before();
+          mbar_arrive(&tempty[buf]);
+        }
+        if (!ok || cols <= 0) continue;
+        if (cols < kHalf) {
+#pragma unroll
+          for (int j = 0; j < kHalf; ++j)
+            if (j >= cols) v[j] = -INFINITY;
+        }
+        const int want = id - first;
+        if (__any_sync(0xffffffffu, want >= 0 && want < cols)) {
+#pragma unroll
+          for (int j = 0; j < kHalf; ++j)
+            if (j == want && want < cols) given = v[j];
+        }
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < kHalf; ++j) top = fmaxf(top, v[j]);
+        a.raise(top);
+        const float sh = a.shift();
+        const u64t shift = pack2(sh, sh);
+        u64t s0 = 0, s1 = 0, e0 = 0, e1 = 0;
+#pragma unroll
+        for (int j = 0; j < kHalf; j += 4) {
+          logprob_terms<true>(v[j], v[j + 1], shift, s0, e0);
+          logprob_terms<true>(v[j + 2], v[j + 3], shift, s1, e1);
+        }
+        float s, t, e, f;
+        unpack2(add2(s0, s1), s, t);
+        unpack2(add2(e0, e1), e, f);
+        a.add(s + t, e + f);
+      }
+      if (!ok) a.hi = NAN;
+      p.part[(long long)(share * 2 + half) * p.row_tiles * kRows + row] = make_float4(a.m, a.hi + a.lo, a.e, given);
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2 * kCols>(tmem);
+  }
+}
+
+// One warp per row joins its shares.
+__global__ void __launch_bounds__(128) lm_logprobs_join_kernel(const float4* __restrict__ part, int parts, int pitch,
+                                                               int T, int V, const int* __restrict__ ids,
+                                                               float* __restrict__ lp, float* __restrict__ entropy) {
+  griddep_wait();
+  griddep_launch();
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= T) return;
+  float m = -INFINITY, given = 0.f;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part[(long long)i * pitch + row].x);
+  m = warp_max(m);
+  double s = 0.0, e = 0.0;
+  for (int i = lane; i < parts; i += 32) {
+    const float4 t = part[(long long)i * pitch + row];
+    const float d = t.x == -INFINITY ? 0.f : fmaxf((t.x - m) * kLog2e, -300.f);
+    const double f = fast_exp2(d);
+    s += f * t.y;
+    e += f * (t.z + t.y * d);
+    given += t.w;  // one share's, the others hold 0
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    e += __shfl_xor_sync(0xffffffffu, e, o);
+    given += __shfl_xor_sync(0xffffffffu, given, o);
+  }
+  if (lane != 0) return;
+  const bool bad = s != s, empty = !bad && s == 0.0;
+  const float log_s = empty ? 0.f : s < 2.0 ? log1pf(float(s - 1.0)) : logf(float(s));
+  const int id = ids[row];
+  entropy[row] = bad ? NAN : empty ? 0.f : float(log_s - e / s * kLn2);
+  lp[row] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (given - (empty ? 0.f : m)) - log_s;
+}
+
+// Shares of a row tile: the split of the vocabulary that leaves the busiest CTA the fewest
+// 64-token units, counting a tile's epilogue and an item's start as one unit each.
+int lm_logprobs_shares(int T, int V, int num_sms) {
+  const int tiles = (T + kRows - 1) / kRows, units = (V + kUnit - 1) / kUnit;
+  long long best_cost = -1;
+  int best = 1;
+  for (int s = 1; s <= std::min(units, num_sms); ++s) {
+    const long long rounds = ((long long)tiles * s + num_sms - 1) / num_sms;
+    const long long cost = rounds * ((units + s - 1) / s + 1);
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+long long lm_logprobs_workspace(int T, int V, int num_sms) {  // float4 elements
+  return 2ll * lm_logprobs_shares(T, V, num_sms) * ((T + kRows - 1) / kRows) * kRows;
+}
+
+void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K, const int* ids,
+                 void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s) {
+  if (T <= 0) return;
+  LmParams p = {};
+  p.T = T;
+  p.V = V;
+  p.K = K;
+  p.row_tiles = (T + kRows - 1) / kRows;
+  p.units = (V + kUnit - 1) / kUnit;
+  p.shares = lm_logprobs_shares(T, V, num_sms);
+  p.ids = ids;
+  p.part = static_cast<float4*>(workspace);
+  p.err = err;
+  CUtensorMap tx, tw;
+  make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, kRows, kBlockK);
+  make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kUnit, kBlockK);
+  set_smem_bytes(lm_logprobs_kernel, kSmem);
+  const int grid = (int)std::min<long long>(num_sms, (long long)p.row_tiles * p.shares);
+  launch_k(lm_logprobs_kernel, dim3(grid), dim3(64 + kEpilogue), kSmem, s, tx, tw, p);
+  launch_k(lm_logprobs_join_kernel, dim3((T + 3) / 4), dim3(128), 0, s, (const float4*)workspace, 2 * p.shares,
+           p.row_tiles * kRows, T, V, ids, lp, entropy);
+}
+
+}  // namespace sp

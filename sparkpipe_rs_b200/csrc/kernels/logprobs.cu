@@ -34,14 +34,13 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "logprobs.cuh"
 #include "pdl.h"
 
 namespace sp {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr double kLn2 = 0.6931471805599453;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 // 64 registers: with 48 the loop spills, with 80 fewer warps hide the exponentials (8,192 rows x
@@ -56,30 +55,7 @@ constexpr int kHot = 512;         // (thread, slot) entries whose batches reach 
 constexpr int kMaxCluster = 8;
 constexpr int kNone = 0x7fffffff;
 
-using u64t = unsigned long long;
-
-// Packed fp32 pairs (one instruction for two).
-SP_DEVI u64t pack2(float a, float b) {
-  u64t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-SP_DEVI void unpack2(u64t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-SP_DEVI u64t add2(u64t a, u64t b) {
-  u64t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-SP_DEVI u64t mul2(u64t a, u64t b) {
-  u64t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-SP_DEVI u64t fma2(u64t a, u64t b, u64t c) {
-  u64t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
+// maxima that keep NaN
 SP_DEVI unsigned max_nan_bf16x2(unsigned a, unsigned b) {
   unsigned r;
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -90,13 +66,6 @@ SP_DEVI unsigned max_nan_f16x2(unsigned a, unsigned b) {
   asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// max that keeps NaN
-SP_DEVI float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // 16 bytes of logits: their values, and the maximum (NaN dropped) of two such vectors.
 template <typename T>
 struct Logits;
@@ -171,46 +140,6 @@ SP_DEVI float batch_max(const uint4 (&v)[kBatch]) {
   return fmaxf(a, b);
 }
 
-// Running sums of a thread: terms 2^u, u = (x - m) log2 e, in hi + lo, and terms 2^u u in e.
-struct Sums {
-  float m = -INFINITY, hi = 0.f, lo = 0.f, e = 0.f;
-
-  SP_DEVI void raise(float top) {  // a larger maximum
-    if (top > m) {
-      const float d = fmaxf((m - top) * kLog2e, -300.f);  // m = -inf: the sums are 0
-      const float w = fast_exp2(d);
-      e = w * fmaf(hi, d, e);
-      hi *= w;
-      lo *= w;
-      m = top;
-    }
-  }
-  SP_DEVI float shift() const { return m == -INFINITY ? 0.f : -m; }  // only -inf so far: u = -inf
-  SP_DEVI void add(float s, float f) {
-    const float t = hi + s, z = t - hi;
-    lo += (hi - (t - z)) + (s - z);
-    hi = t;
-    e += f;
-  }
-};
-
-// Adds the terms of two logits. CLAMP bounds u below, so that 0 * u stays 0 for -inf (and for
-// differences past fp32's range).
-template <bool CLAMP>
-SP_DEVI void term2(float a, float b, u64t shift, u64t& s, u64t& e) {
-  u64t u = mul2(add2(pack2(a, b), shift), pack2(kLog2e, kLog2e));
-  float u0, u1;
-  unpack2(u, u0, u1);
-  if (CLAMP) {
-    u0 = max_nan(u0, -200.f);
-    u1 = max_nan(u1, -200.f);
-    u = pack2(u0, u1);
-  }
-  const u64t p = pack2(fast_exp2(u0), fast_exp2(u1));
-  s = add2(s, p);
-  e = fma2(p, u, e);
-}
-
 // The sums of a batch's terms. Beside a maximum of ordinary size (CLAMP false) very small
 // logits are raised, two in one instruction, so that -inf needs no care further on.
 template <typename T, bool CLAMP>
@@ -227,8 +156,8 @@ SP_DEVI void batch_terms(const uint4 (&v)[kBatch], float shift, float& s, float&
       float f0, f1, f2, f3;
       values2<T>(r, j, f0, f1);
       values2<T>(r, j + 1, f2, f3);
-      term2<CLAMP>(f0, f1, sh, s0, e0);
-      term2<CLAMP>(f2, f3, sh, s1, e1);
+      logprob_terms<CLAMP>(f0, f1, sh, s0, e0);
+      logprob_terms<CLAMP>(f2, f3, sh, s1, e1);
     }
   }
   float p, q;
@@ -442,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const int nb = (part.v1 - part.v0 + kBatch * kThreads - 1) / (kBatch * kThreads);
   const int per_slot = (nb + kSlots - 1) / kSlots;
 
-  Sums a;
+  LogprobSums a;
   float slot_max = -INFINITY;
   int slot = 0, left = per_slot;
   auto take = [&](uint4 (&v)[kBatch]) {
@@ -494,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     a.raise(top);
     const float shift = a.shift();
     u64t s0 = 0, e0 = 0;
-    term2<true>(one, two, pack2(shift, shift), s0, e0);
+    logprob_terms<true>(one, two, pack2(shift, shift), s0, e0);
     float p, q, f, g;
     unpack2(s0, p, q);
     unpack2(e0, f, g);

@@ -1118,6 +1118,31 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
   return {lp, entropy, top_lp, top_ids};
 }
 
+std::tuple<Tensor, Tensor> linear_logprobs(const Tensor& x, const Tensor& w, const Tensor& ids) {
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "linear_logprobs: x [T, K] and w [V, K]");
+  CHECK_BF16(x); CHECK_BF16(w); CHECK_I32(ids); CHECK_CONTIG(ids);
+  TORCH_CHECK(ids.dim() == 1 && ids.size(0) == x.size(0), "linear_logprobs: ids must be [T], one per row of x");
+  const int64_t T = x.size(0), V = w.size(0), K = x.size(1);
+  TORCH_CHECK(T == 0 || (V >= 1 && K >= 1), "linear_logprobs: no columns");
+  TORCH_CHECK(K % 8 == 0, "linear_logprobs: K must be a multiple of 8");
+  auto rows_ok = [](const Tensor& t) {
+    return (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
+           (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  };
+  TORCH_CHECK(rows_ok(x) && rows_ok(w), "linear_logprobs: x and w must be row-major with 16-byte aligned rows");
+  TORCH_CHECK(T <= INT_MAX / 4 && V <= INT_MAX / 4 && K <= INT_MAX / 4, "linear_logprobs: too large");
+  CHECK_CUDA(x); CHECK_ON(x, w); CHECK_ON(x, ids);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  const Tensor lp = at::empty({T}, f32), entropy = at::empty({T}, f32);
+  if (T == 0) return {lp, entropy};
+  const Tensor work = at::empty({4 * sp::lm_logprobs_workspace((int)T, (int)V, num_sms())}, f32);
+  sp::lm_logprobs(x.data_ptr(), T > 1 ? x.stride(0) : (K + 7) / 8 * 8, w.data_ptr(), V > 1 ? w.stride(0) : (K + 7) / 8 * 8,
+                  (int)T, (int)V, (int)K, ids.data_ptr<int>(), work.data_ptr(), lp.data_ptr<float>(),
+                  entropy.data_ptr<float>(), err_word(), num_sms(), stream());
+  return {lp, entropy};
+}
+
 // One plane of a paged cache [layers, slots, row]; any layer stride, rows and slots dense.
 sp::PagePlane page_plane(const Tensor& t, int64_t block_size, const char* who) {
   TORCH_CHECK(t.dim() == 3 && t.size(2) >= 1 && (t.stride(2) == 1 || t.size(2) == 1) &&
@@ -1307,6 +1332,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("phase_mark", &phase_mark);
   m.def("kv_blocks_copy", &kv_blocks_copy);
   m.def("token_logprobs", &token_logprobs);
+  m.def("linear_logprobs", &linear_logprobs);
   m.def("copy_pages", &copy_pages);
   m.def("fork_pages", &fork_pages);
   m.def("reserve_pages", &reserve_pages);

@@ -629,22 +629,11 @@ def linear_logprobs(x, w, ids):
     """Log probabilities of given tokens and entropy of softmax(x @ w.T), without keeping
     the logits: prompt scoring straight from hidden states and the LM head.
 
-    ``x`` [T, K] (row-major view) and ``w`` [V, K] bf16, K a multiple of 8; ``ids`` int32
-    [T] (-1: nothing asked, 0). Logits are the fp32 accumulators, not rounded to bf16.
-    Returns (logprobs [T], entropy [T]) fp32."""
-    T, V = x.shape[0], w.shape[0]
-    if ids.shape != (T,):
-        raise ValueError("linear_logprobs: ids must be [T], one per row of x")
-    f32 = dict(dtype=torch.float32, device=x.device)
-    lp, entropy = torch.empty(T, **f32), torch.empty(T, **f32)
-    rows = max(1, min(T, (1 << 28) // max(V, 1)))
-    buf = torch.empty(rows, -(-V // 4) * 4, **f32)
-    for r in range(0, T, rows):
-        n = min(rows, T - r)
-        logits = linear(x[r:r + n], w, out=buf[:n, :V], splits=1)
-        part = token_logprobs(logits, ids[r:r + n])
-        lp[r:r + n] = part.logprobs
-        entropy[r:r + n] = part.entropy
+    ``x`` [T, K] and ``w`` [V, K] bf16, row-major with 16-byte aligned rows, K a multiple of
+    8; ``ids`` int32 [T], -1 and ids outside [0, V) as in ``token_logprobs``. Logits are the
+    fp32 accumulators, not rounded to bf16. Returns (logprobs [T], entropy [T]) fp32."""
+    lp, entropy = kernels().linear_logprobs(x, w, ids)
+    _count(2 if x.shape[0] else 0)
     return lp, entropy
 
 
