@@ -35,22 +35,29 @@ namespace sp {
 
 namespace {
 
-constexpr int kRows = 128;       // rows of an item
+constexpr int kRows = 128;       // rows of a CTA's item
 constexpr int kCols = 256;       // logits of a tile's row
-constexpr int kUnit = 64;        // tokens of a unit: rows of one TMA box of w
+constexpr int kBox = 64;         // rows of a TMA box of w
 constexpr int kBlockK = 64;
 constexpr int kSegBlocks = 16;   // K blocks of a segment
-constexpr int kStages = 4;
 constexpr int kXBytes = kRows * kBlockK * 2;
-constexpr int kBoxBytes = kUnit * kBlockK * 2;
-constexpr int kStageBytes = kXBytes + kCols / kUnit * kBoxBytes;
-constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+constexpr int kBoxBytes = kBox * kBlockK * 2;
 constexpr int kHalf = 128;       // columns of an epilogue thread
 constexpr int kEpilogue = 256;   // epilogue threads
 
+// CTAs = 2: a pair of CTAs shares a tile of 256 rows x 256 logits, each loads half of w's rows.
+template <int CTAS>
+struct Lm {
+  static constexpr int kUnit = kBox * CTAS;         // tokens of a unit of the vocabulary
+  static constexpr int kTile = kCols / kUnit;       // units of a tile = boxes of w that a CTA loads
+  static constexpr int kStageBytes = kXBytes + kTile * kBoxBytes;
+  static constexpr int kStages = CTAS == 2 ? 6 : 4;
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+};
+
 struct LmParams {
   int T, V, K;
-  int row_tiles, units, shares;  // row tiles, 64-token units, shares of a row tile
+  int row_tiles, units, shares;  // row tiles, units of the vocabulary, shares of a row tile
   const int* ids;
   float4* part;                  // [shares * 2][row_tiles * 128]: m, S, E (log2 units), the given token's logit
   int* err;
@@ -63,9 +70,12 @@ SP_DEVI void share_units(const LmParams& p, int share, int& u0, int& u1) {
 
 }  // namespace
 
+template <int CTAS>
 __global__ void __launch_bounds__(64 + kEpilogue, 1)
     lm_logprobs_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                        const LmParams p) {
+  using C = Lm<CTAS>;
+  constexpr int kStages = C::kStages, kStageBytes = C::kStageBytes, kTile = C::kTile, kUnit = C::kUnit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
@@ -75,6 +85,7 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? (int)cluster_ctarank() : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -82,7 +93,7 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], kEpilogue);
+      mbar_init(&tempty[i], CTAS * kEpilogue / 32);
     }
     *s_err = 0;
     fence_mbarrier_init();
@@ -90,29 +101,37 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
     prefetch_tmap(&tmW);
   }
   if (warp == 1) {
-    tmem_alloc<2 * kCols>(tmem_slot);
-    tmem_relinquish();
+    if (CTAS == 2) {
+      tmem_alloc_pair<2 * kCols>(tmem_slot);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc<2 * kCols>(tmem_slot);
+      tmem_relinquish();
+    }
     tc_fence_before();
   }
-  __syncthreads();
+  if (CTAS == 2) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   griddep_launch();
   griddep_wait();
   const uint32_t tmem = *tmem_slot;
   const int items = p.row_tiles * p.shares;
   const int blocks = (p.K + kBlockK - 1) / kBlockK;
+  const int item0 = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 0) {
     if (lane == 0) {
       const uint64_t once = policy_evict_first();  // with one row tile, w only passes through L2
       int it = 0;
       bool ok = true;
-      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      for (int item = item0; ok && item < items; item += step) {
         int u0, u1;
         share_units(p, item / p.row_tiles, u0, u1);
-        const int row = (item % p.row_tiles) * kRows;
-        for (; ok && u0 < u1; u0 += kCols / kUnit) {
-          const int n = min(kCols / kUnit, u1 - u0);
+        const int row = ((item % p.row_tiles) * CTAS + rank) * kRows;
+        for (; ok && u0 < u1; u0 += kTile) {
+          const int n = min(kTile, u1 - u0);
+          const int col = u0 * kUnit + rank * n * kBox;  // a pair splits the tile's rows of w
           for (int kb = 0; kb < blocks; ++kb, ++it) {
             const int s = it % kStages;
             if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutProducer)) {
@@ -120,29 +139,37 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
               break;
             }
             uint8_t* at = smem + s * kStageBytes;
-            mbar_arrive_expect_tx(&full[s], kXBytes + n * kBoxBytes);
-            tma_load_2d(at, &tmX, &full[s], kb * kBlockK, row);
-            for (int i = 0; i < n; ++i) {
-              uint8_t* box = at + kXBytes + i * kBoxBytes;
-              if (p.row_tiles == 1) tma_load_2d_hint(box, &tmW, &full[s], kb * kBlockK, (u0 + i) * kUnit, once);
-              else tma_load_2d(box, &tmW, &full[s], kb * kBlockK, (u0 + i) * kUnit);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (kXBytes + n * kBoxBytes));
+            if (CTAS == 2) {
+              const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+              tma_load_2d_pair(at, &tmX, bar, kb * kBlockK, row);
+              for (int i = 0; i < n; ++i)
+                tma_load_2d_pair(at + kXBytes + i * kBoxBytes, &tmW, bar, kb * kBlockK, col + i * kBox);
+            } else {
+              tma_load_2d(at, &tmX, &full[s], kb * kBlockK, row);
+              for (int i = 0; i < n; ++i) {
+                uint8_t* box = at + kXBytes + i * kBoxBytes;
+                if (p.row_tiles == 1) tma_load_2d_hint(box, &tmW, &full[s], kb * kBlockK, col + i * kBox, once);
+                else tma_load_2d(box, &tmW, &full[s], kb * kBlockK, col + i * kBox);
+              }
             }
           }
         }
       }
-      // loads in flight land before the CTA gives up its memory
-      for (int j = max(0, it - kStages); j < it && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
+      // loads in flight land before the CTA gives up its memory (a pair's count on its first CTA)
+      if (rank == 0)
+        for (int j = max(0, it - kStages); j < it && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int it = 0, tc = 0;
       bool ok = true;
-      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      for (int item = item0; ok && item < items; item += step) {
         int u0, u1;
         share_units(p, item / p.row_tiles, u0, u1);
-        for (; ok && u0 < u1; u0 += kCols / kUnit) {
-          const uint32_t idesc = idesc_bf16_f32(kRows, min(kCols / kUnit, u1 - u0) * kUnit);
+        for (; ok && u0 < u1; u0 += kTile) {
+          const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, min(kTile, u1 - u0) * kUnit);
           for (int kb = 0; kb < blocks; ++kb, ++it) {
             const int buf = tc & 1;
             if (kb % kSegBlocks == 0) {
@@ -155,13 +182,20 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
             const uint32_t at = smem_u32(smem + s * kStageBytes);
             const uint64_t a = sdesc_kmajor_sw128(at), b = sdesc_kmajor_sw128(at + kXBytes);
 #pragma unroll
-            for (int k = 0; k < kBlockK / 16; ++k)
-              umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, (kb % kSegBlocks > 0 || k > 0) ? 1u : 0u);
-            umma_commit(&empty[s]);
-            if (kb % kSegBlocks == kSegBlocks - 1 || kb == blocks - 1) {
-              umma_commit(&tfull[buf]);
-              ++tc;
+            for (int k = 0; k < kBlockK / 16; ++k) {
+              const uint32_t more = (kb % kSegBlocks > 0 || k > 0) ? 1u : 0u;
+              if (CTAS == 2) umma_f16_pair(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
+              else umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
             }
+            const bool last = kb % kSegBlocks == kSegBlocks - 1 || kb == blocks - 1;
+            if (CTAS == 2) {
+              umma_commit_pair(&empty[s]);
+              if (last) umma_commit_pair(&tfull[buf]);
+            } else {
+              umma_commit(&empty[s]);
+              if (last) umma_commit(&tfull[buf]);
+            }
+            if (last) ++tc;
           }
         }
       }
@@ -173,15 +207,15 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
     const uint32_t mine = tmem + (uint32_t(q * 32) << 16) + half * kHalf;
     int tc = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    for (int item = item0; item < items; item += step) {
       const int share = item / p.row_tiles;
       int u0, u1;
       share_units(p, share, u0, u1);
-      const int row = (item % p.row_tiles) * kRows + m;
+      const int row = ((item % p.row_tiles) * CTAS + rank) * kRows + m;
       const int id = row < p.T ? p.ids[row] : -1;
       LogprobSums a;
       float given = 0.f;
-      for (; ok && u0 < u1; u0 += kCols / kUnit) {
+      for (; ok && u0 < u1; u0 += kTile) {
         const int first = u0 * kUnit + half * kHalf;
         // columns of this thread: up to the share's end and the vocabulary's
         const int cols = min(kHalf, min(u1 * kUnit, p.V) - first);
@@ -213,7 +247,11 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
             }
           }
           tc_fence_before();
-          mbar_arrive(&tempty[buf]);
+          __syncwarp();
+          if (lane == 0) {
+            if (CTAS == 2) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[buf]), 0));
+            else mbar_arrive(&tempty[buf]);
+          }
         }
         if (!ok || cols <= 0) continue;
         if (cols < kHalf) {
@@ -245,13 +283,15 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
         a.add(s + t, e + f);
       }
       if (!ok) a.hi = NAN;
-      p.part[(long long)(share * 2 + half) * p.row_tiles * kRows + row] = make_float4(a.m, a.hi + a.lo, a.e, given);
+      p.part[(long long)(share * 2 + half) * p.row_tiles * CTAS * kRows + row] = make_float4(a.m, a.hi + a.lo, a.e, given);
     }
   }
-  __syncthreads();
+  if (CTAS == 2) cluster_sync();  // a pair's shared memory serves both CTAs
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<2 * kCols>(tmem);
+    if (CTAS == 2) tmem_dealloc_pair<2 * kCols>(tmem);
+    else tmem_dealloc<2 * kCols>(tmem);
   }
 }
 
@@ -289,48 +329,90 @@ __global__ void __launch_bounds__(128) lm_logprobs_join_kernel(const float4* __r
   lp[row] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (given - (empty ? 0.f : m)) - log_s;
 }
 
-// Shares of a row tile: the split of the vocabulary that leaves the busiest CTA the fewest
-// 64-token units, counting a tile's epilogue and an item's start as one unit each.
-int lm_logprobs_shares(int T, int V, int num_sms) {
-  const int tiles = (T + kRows - 1) / kRows, units = (V + kUnit - 1) / kUnit;
-  long long best_cost = -1;
-  int best = 1;
-  for (int s = 1; s <= std::min(units, num_sms); ++s) {
-    const long long rounds = ((long long)tiles * s + num_sms - 1) / num_sms;
-    const long long cost = rounds * ((units + s - 1) / s + 1);
-    if (best_cost < 0 || cost < best_cost) {
-      best_cost = cost;
-      best = s;
+namespace {
+
+struct LmPlan {
+  int ctas, row_tiles, units, shares;
+};
+
+// CTA pairs from two row tiles on. The vocabulary's shares per row tile are as many as leave
+// the busiest CTA the fewest units, counting an item's start as one more.
+LmPlan lm_plan(int T, int V, int num_sms) {
+  LmPlan l;
+  l.ctas = T > kRows ? 2 : 1;
+  if (const char* e = getenv("LM_CTAS")) l.ctas = atoi(e);
+  l.row_tiles = (T + kRows * l.ctas - 1) / (kRows * l.ctas);
+  l.units = (V + kBox * l.ctas - 1) / (kBox * l.ctas);
+  const int workers = num_sms / l.ctas;
+  long long best = -1;
+  for (int s = 1; s <= std::min(l.units, workers); ++s) {
+    const long long rounds = ((long long)l.row_tiles * s + workers - 1) / workers;
+    const long long cost = rounds * ((l.units + s - 1) / s + 1);
+    if (best < 0 || cost < best) {
+      best = cost;
+      l.shares = s;
     }
   }
-  return best;
+  return l;
 }
 
-long long lm_logprobs_workspace(int T, int V, int num_sms) {  // float4 elements
-  return 2ll * lm_logprobs_shares(T, V, num_sms) * ((T + kRows - 1) / kRows) * kRows;
+template <int CTAS>
+void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, const LmParams& p, int num_sms,
+               cudaStream_t s) {
+  auto kern = lm_logprobs_kernel<CTAS>;
+  set_smem_bytes(kern, Lm<CTAS>::kSmem);
+  prefer_max_smem_carveout(reinterpret_cast<const void*>(kern));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attrs[2];
+  cfg.gridDim = dim3(CTAS * (unsigned)std::min<long long>(num_sms / CTAS, (long long)l.row_tiles * l.shares));
+  cfg.blockDim = dim3(64 + kEpilogue);
+  cfg.dynamicSmemBytes = Lm<CTAS>::kSmem;
+  cfg.stream = s;
+  cfg.attrs = attrs;
+  if (CTAS == 2) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = 2;
+    attrs[cfg.numAttrs].val.clusterDim.y = 1;
+    attrs[cfg.numAttrs].val.clusterDim.z = 1;
+    cfg.numAttrs += 1;
+  }
+  if (pdl_enabled()) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs += 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, p);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("lm_logprobs launch failed: ") + cudaGetErrorString(e));
+}
+
+}  // namespace
+
+long long lm_logprobs_workspace(int T, int V, int num_sms) {
+  const LmPlan l = lm_plan(T, V, num_sms);
+  return 2ll * l.shares * l.row_tiles * l.ctas * kRows;
 }
 
 void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K, const int* ids,
                  void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s) {
   if (T <= 0) return;
+  const LmPlan l = lm_plan(T, V, num_sms);
   LmParams p = {};
   p.T = T;
   p.V = V;
   p.K = K;
-  p.row_tiles = (T + kRows - 1) / kRows;
-  p.units = (V + kUnit - 1) / kUnit;
-  p.shares = lm_logprobs_shares(T, V, num_sms);
+  p.row_tiles = l.row_tiles;
+  p.units = l.units;
+  p.shares = l.shares;
   p.ids = ids;
   p.part = static_cast<float4*>(workspace);
   p.err = err;
   CUtensorMap tx, tw;
   make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, kRows, kBlockK);
-  make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kUnit, kBlockK);
-  set_smem_bytes(lm_logprobs_kernel, kSmem);
-  const int grid = (int)std::min<long long>(num_sms, (long long)p.row_tiles * p.shares);
-  launch_k(lm_logprobs_kernel, dim3(grid), dim3(64 + kEpilogue), kSmem, s, tx, tw, p);
+  make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
+  if (l.ctas == 2) launch_lm<2>(l, tx, tw, p, num_sms, s);
+  else launch_lm<1>(l, tx, tw, p, num_sms, s);
   launch_k(lm_logprobs_join_kernel, dim3((T + 3) / 4), dim3(128), 0, s, (const float4*)workspace, 2 * p.shares,
-           p.row_tiles * kRows, T, V, ids, lp, entropy);
+           p.row_tiles * l.ctas * kRows, T, V, ids, lp, entropy);
 }
 
 }  // namespace sp
