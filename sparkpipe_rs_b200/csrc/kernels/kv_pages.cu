@@ -17,9 +17,12 @@
 //                     every layer and plane.
 //
 // The index kernels run in one CTA where an order is needed (which row gets which page):
-// tables and counts are a few KB. The copies are bound by memory: every thread keeps four
-// 16-byte loads in flight, and the work is cut into 16 KB pieces so that one page of one
-// layer already spreads over several SMs.
+// tables and counts are a few KB, and what they cost is the latency of reading them. The
+// copies are bound by memory: bulk copies through shared memory, in pieces of a quarter of
+// a page or so, move 400 pages x 27 layers (0.8 GB) at 6.06 TB/s, 94% of the measured copy
+// bandwidth; the same copies by 16-byte loads and stores of 2,048 threads per SM reached
+// 5.34 TB/s. Three CTAs per SM keep one thread's issue from bounding small pieces: partly
+// filled pages of 256 rows 40.6 us, against 47.5 us with two larger rings.
 //
 // Reference: the page / block-table bookkeeping of the KV arena
 // (crates/spark-abi/vendor/sparkpipe/include/sparkpipe/spark_kv_cache.h:227-300); sharing
@@ -37,30 +40,32 @@ namespace sp {
 
 namespace {
 
-constexpr int kCopyThreads = 256;
-constexpr int kPiece = 4 * kCopyThreads;  // vectors of one piece: four per thread
+constexpr int kCopyThreads = 128;
+constexpr int kStages = 4, kStageBytes = 18432;  // a copy CTA's ring: 72 KB, three per SM
+constexpr int kCopyCtas = 3;
 constexpr int kIndexThreads = 1024;
+constexpr int kGrants = 4096;   // pages granted in one call that fit in shared memory
+constexpr int kNearRefs = 8192; // page counts that do
 
 // Exclusive prefix sum of one value per thread over the CTA; every thread gets the total.
 SP_DEVI int block_scan(int v, int* total, int* warp_sums) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int x = v;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  auto scan = [&](int x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const int x = scan(v);
   __syncthreads();  // the previous scan's readers are done with warp_sums
   if (lane == 31) warp_sums[w] = x;
   __syncthreads();
-  int base = 0, all = 0;
-  for (int i = 0; i < warps; ++i) {
-    const int t = warp_sums[i];
-    if (i < w) base += t;
-    all += t;
-  }
-  *total = all;
-  return base + x - v;
+  const int sums = scan(lane < (int)blockDim.x >> 5 ? warp_sums[lane] : 0);  // in every warp
+  *total = __shfl_sync(0xffffffffu, sums, 31);
+  const int base = __shfl_sync(0xffffffffu, sums, w > 0 ? w - 1 : 0);
+  return (w > 0 ? base : 0) + x - v;
 }
 
 SP_DEVI int pages_of(int tokens, int block_size) { return tokens <= 0 ? 0 : (tokens - 1) / block_size + 1; }
@@ -105,30 +110,37 @@ void pages_fork(const int* table, int rows, int cols, const int* lens, const int
 
 // ------------------------------------------------------------------ reserve
 // One CTA. Phase 1: what each row needs, and its place among the needs of the rows before
-// it; phase 2: the lowest free pages, as many as are needed; phase 3: grants. `free_list`
-// holds [pages] ids; `work` gets the copy list, (source, destination, tokens) records, and
-// `copies` its length.
+// it; phase 2: the lowest free pages, as many as are needed; phase 3: grants. The counts of up
+// to kNearRefs pages and up to kGrants granted pages stay in shared memory, so that a beam
+// step pays two dependent reads of memory (a row's length, its last page); larger caches read
+// refs again, larger grants go through `free_list` [pages]. `work` gets the copy list, (source,
+// destination, tokens) records, and `copies` its length.
 __global__ void __launch_bounds__(kIndexThreads)
     pages_reserve_kernel(int* __restrict__ table, int rows, int cols, const int* __restrict__ lens,
-                         const int* __restrict__ row_tokens, int tokens, int* __restrict__ refs, int pages,
-                         int block_size, int* __restrict__ free_list, int* __restrict__ work, int* __restrict__ copies,
-                         int* __restrict__ short_by) {
+                         const int* __restrict__ row_tokens, int tokens, int* refs, int pages, int block_size,
+                         int* free_list, int* __restrict__ work, int* __restrict__ copies, int* __restrict__ short_by) {
   extern __shared__ int smem[];
-  int* tail = smem;          // [rows] last page if other rows hold it too, else -1
-  int* start = smem + rows;  // [rows] pages granted to the rows before
-  int* need = start + rows;  // [rows]
+  int* tail = smem;             // [rows] last page if other rows hold it too, else -1
+  int* start = tail + rows;     // [rows] pages granted to the rows before
+  int* need = start + rows;     // [rows]
+  int* grants = need + rows;    // [kGrants]
+  int* near = grants + kGrants; // [min(pages, kNearRefs)]
   __shared__ int warp_sums[32];
   __shared__ int s_copies;
   griddep_wait();
   griddep_launch();
+  const bool in_near = pages <= kNearRefs;
+  const int* counts = in_near ? near : refs;  // as they were before the call
   if (threadIdx.x == 0) s_copies = 0;
+  if (in_near)
+    for (int p = threadIdx.x; p < pages; p += blockDim.x) near[p] = refs[p];
   for (int b = threadIdx.x; b < rows; b += blockDim.x) {
     const int len = lens[b];
     const int want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
     int t = -1;
     if (want > 0 && len > 0 && len % block_size != 0 && len / block_size < cols) {
       t = table[(long long)b * cols + len / block_size];
-      if (t < 0 || t >= pages || refs[t] <= 1) t = -1;
+      if (t < 0 || t >= pages) t = -1;
     }
     tail[b] = t;
   }
@@ -142,9 +154,13 @@ __global__ void __launch_bounds__(kIndexThreads)
       const int want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
       const int t = tail[b];
       if (t >= 0) {
+        // the rows before this one with the same last page will have left it
+        const int held = counts[t];
         int earlier = 0;
-        for (int q = 0; q < b; ++q) earlier += tail[q] == t;
-        if (refs[t] - earlier > 1) n = 1;
+        if (held > 1)
+#pragma unroll 8
+          for (int q = 0; q < b; ++q) earlier += tail[q] == t;
+        n = held - earlier > 1;
       }
       if (want > 0) {
         const long long end = (long long)len + want;
@@ -160,13 +176,14 @@ __global__ void __launch_bounds__(kIndexThreads)
     carry += total;
   }
   // free pages, lowest first
+  int* list = carry <= kGrants ? grants : free_list;
   int found = 0;
   for (int p0 = 0; p0 < pages && found < carry; p0 += blockDim.x) {
     const int p = p0 + threadIdx.x;
-    const int is_free = p < pages && refs[p] <= 0;
+    const int is_free = p < pages && counts[p] <= 0;
     int total;
     const int at = found + block_scan(is_free, &total, warp_sums);
-    if (is_free && at < carry) free_list[at] = p;
+    if (is_free && at < carry) list[at] = p;
     found += total;
   }
   __syncthreads();
@@ -184,9 +201,8 @@ __global__ void __launch_bounds__(kIndexThreads)
     int fresh = 0;
     for (int c = first; c < last; ++c) fresh += t[c] < 0;
     if (n > fresh) {  // the shared last page comes first
-      const int page = free_list[g++];
-      const int i = atomicAdd(&s_copies, 1);
-      int* rec = work + 3 * i;
+      const int page = list[g++];
+      int* rec = work + 3 * atomicAdd(&s_copies, 1);
       rec[0] = tail[b];
       rec[1] = page;
       rec[2] = len % block_size;
@@ -196,7 +212,7 @@ __global__ void __launch_bounds__(kIndexThreads)
     }
     for (int c = first; c < last; ++c)
       if (t[c] < 0) {
-        const int page = free_list[g++];
+        const int page = list[g++];
         refs[page] = 1;
         t[c] = page;
       }
@@ -209,8 +225,10 @@ void pages_reserve(int* table, int rows, int cols, const int* lens, const int* r
                    int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s) {
   if (rows <= 0) return;
   if (rows > kPagesMaxRows) throw std::runtime_error("pages_reserve: too many rows");
-  launch_k(pages_reserve_kernel, dim3(1), dim3(kIndexThreads), sizeof(int) * 3 * rows, s, table, rows, cols, lens,
-           row_tokens, tokens, refs, pages, block_size, free_list, work, copies, short_by);
+  auto smem = [](int rows, int pages) { return (int)sizeof(int) * (3 * rows + kGrants + std::min(pages, kNearRefs)); };
+  set_smem_bytes(pages_reserve_kernel, smem(kPagesMaxRows, kNearRefs));
+  launch_k(pages_reserve_kernel, dim3(1), dim3(kIndexThreads), smem(rows, pages <= kNearRefs ? pages : 0), s, table,
+           rows, cols, lens, row_tokens, tokens, refs, pages, block_size, free_list, work, copies, short_by);
 }
 
 // ------------------------------------------------------------------ free
@@ -343,81 +361,144 @@ void pages_pairs(const int* src, const int* dst, int n, int pages, int block_siz
            err);
 }
 
+// Every thread that runs the small or unaligned part of a copy moves 4-byte words.
 struct CopyPlane {
   char* base;
   long long layer_stride;  // bytes
-  int page_bytes, token_bytes, pieces;
+  int page_bytes, token_bytes;
 };
 
-// Persistent CTAs over (pair, layer, piece) units, pieces of both planes one after the
-// other. V is the access width: 16 bytes, or 4 where a plane's addresses are only that
-// aligned. A pair's token count bounds its bytes (a last page is copied as far as its row
-// has tokens). The first threads also pass a table through the page map of a compaction.
-template <typename V>
-__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const int* __restrict__ work,
-                                                                  const int* __restrict__ copies, int layers,
-                                                                  CopyPlane a, CopyPlane b, int* __restrict__ table,
-                                                                  long long entries, const int* __restrict__ page_map,
-                                                                  int pages) {
+SP_DEVI void copy_words(const CopyPlane& p, int layer, int src, int dst, int from, int to, int first, int step) {
+  const long long off = layer * p.layer_stride;
+  const int* s = reinterpret_cast<const int*>(p.base + off + (long long)src * p.page_bytes);
+  int* d = reinterpret_cast<int*>(p.base + off + (long long)dst * p.page_bytes);
+#pragma unroll 4
+  for (int w = from / 4 + first; w < to / 4; w += step) d[w] = s[w];
+}
+
+// A table's entries through the page map of a compaction.
+SP_DEVI void remap_table(int* table, long long entries, const int* page_map, int pages) {
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < entries;
+       i += (long long)gridDim.x * blockDim.x) {
+    const int e = table[i];
+    if (e >= 0 && e < pages) table[i] = page_map[e];
+  }
+}
+
+SP_DEVI void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+// Units are (pair, layer, piece of the first plane), dealt to the CTAs in turn. One thread moves
+// them through a ring of shared memory with bulk copies: the load of a unit goes out while the
+// one before it is stored. The other warps move the second plane (block scales, a sixtieth
+// of the bytes) and what a token count leaves of 16 bytes. Pairs carry a token count because a
+// last page is copied as far as its row has tokens.
+__global__ void __launch_bounds__(kCopyThreads)
+    pages_copy_kernel(const int* __restrict__ work, const int* __restrict__ copies, int layers, CopyPlane a,
+                      CopyPlane b, int pieces, int piece_bytes, int* __restrict__ table, long long entries,
+                      const int* __restrict__ page_map, int pages, int* err) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kStages];
+  __shared__ int s_err;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
+    s_err = 0;
+    fence_mbarrier_init();
+  }
   griddep_wait();
   griddep_launch();
-  if (table)
-    for (long long i = (long long)blockIdx.x * kCopyThreads + threadIdx.x; i < entries;
-         i += (long long)gridDim.x * kCopyThreads) {
-      const int e = table[i];
-      if (e >= 0 && e < pages) table[i] = page_map[e];
+  if (table) remap_table(table, entries, page_map, pages);
+  const int rows = *copies * layers;  // (pair, layer)
+  if (threadIdx.x >= 32) {
+    const int lane = threadIdx.x & 31, per_cta = kCopyThreads / 32 - 1;
+    for (int q = blockIdx.x * per_cta + (threadIdx.x >> 5) - 1; q < rows; q += gridDim.x * per_cta) {
+      const int c = q / layers, layer = q - c * layers;
+      const int src = work[3 * c], dst = work[3 * c + 1], tokens = work[3 * c + 2];
+      const int end = tokens * a.token_bytes;
+      copy_words(a, layer, src, dst, end & ~15, end, lane, 32);
+      if (b.base) copy_words(b, layer, src, dst, 0, tokens * b.token_bytes, lane, 32);
     }
-  const int per_page = a.pieces + b.pieces;
-  const long long units = (long long)*copies * layers * per_page;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int piece = int(u % per_page);
-    const long long q = u / per_page;
-    const int layer = int(q % layers), i = int(q / layers);
-    const CopyPlane& pl = piece < a.pieces ? a : b;
-    const int src = work[3 * i], dst = work[3 * i + 1];
-    const int bytes = work[3 * i + 2] * pl.token_bytes;
-    const int v0 = (piece < a.pieces ? piece : piece - a.pieces) * kPiece + threadIdx.x;
-    const char* from = pl.base + layer * pl.layer_stride + (long long)src * pl.page_bytes;
-    char* to = pl.base + layer * pl.layer_stride + (long long)dst * pl.page_bytes;
-    const int whole = bytes / (int)sizeof(V);
-    V v[4];
+    return;
+  }
+  if (threadIdx.x != 0) return;
+  const int units = rows * pieces;
+  const int n = units <= (int)blockIdx.x ? 0 : (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  char* to[kStages];
+  int bytes[kStages];
+  bool ok = true;
+  for (int i0 = 0; i0 < n + 1; i0 += kStages) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v0 + j * kCopyThreads < whole) v[j] = reinterpret_cast<const V*>(from)[v0 + j * kCopyThreads];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = v0 + j * kCopyThreads;
-      if (at < whole) {
-        reinterpret_cast<V*>(to)[at] = v[j];
-      } else if (at == whole) {  // the words of a token count that does not fill a vector
-        for (int w = whole * (int)sizeof(V); w < bytes; w += 4)
-          *reinterpret_cast<int*>(to + w) = *reinterpret_cast<const int*>(from + w);
+    for (int st = 0; st < kStages; ++st) {
+      const int i = i0 + st;
+      if (i < n) {
+        // the store that last read this stage: all but the youngest kStages - 2 have been read
+        if (i >= kStages) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStages - 2) : "memory");
+        const int u = blockIdx.x + i * gridDim.x;
+        const int q = u / pieces, at = (u - q * pieces) * piece_bytes;
+        const int c = q / layers, layer = q - c * layers;
+        const long long off = layer * a.layer_stride + at;
+        to[st] = a.base + off + (long long)work[3 * c + 1] * a.page_bytes;
+        bytes[st] = max(0, min(piece_bytes, (work[3 * c + 2] * a.token_bytes & ~15) - at));
+        mbar_arrive_expect_tx(&full[st], bytes[st]);
+        if (bytes[st])
+          bulk_load(ring + st * kStageBytes, a.base + off + (long long)work[3 * c] * a.page_bytes, bytes[st], &full[st]);
+      }
+      constexpr int kPrev = kStages - 1;
+      const int j = i - 1, ps = (st + kPrev) % kStages;
+      if (j >= 0 && j < n) {
+        ok = ok && mbar_wait(&full[ps], (j / kStages) & 1, &s_err, err, kErrWaitTimeoutProducer);
+        if (ok && bytes[ps]) bulk_store(to[ps], ring + ps * kStageBytes, bytes[ps]);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
+  }
+  for (int j = max(0, n - kStages); j < n && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// Planes whose pages are not 16-byte aligned: a CTA per (pair, layer).
+__global__ void __launch_bounds__(kCopyThreads)
+    pages_copy_words_kernel(const int* __restrict__ work, const int* __restrict__ copies, int layers, CopyPlane a,
+                            CopyPlane b, int* __restrict__ table, long long entries, const int* __restrict__ page_map,
+                            int pages) {
+  griddep_wait();
+  griddep_launch();
+  if (table) remap_table(table, entries, page_map, pages);
+  const int rows = *copies * layers;
+  for (int q = blockIdx.x; q < rows; q += gridDim.x) {
+    const int c = q / layers, layer = q - c * layers;
+    const int src = work[3 * c], dst = work[3 * c + 1], tokens = work[3 * c + 2];
+    copy_words(a, layer, src, dst, 0, tokens * a.token_bytes, threadIdx.x, kCopyThreads);
+    if (b.base) copy_words(b, layer, src, dst, 0, tokens * b.token_bytes, threadIdx.x, kCopyThreads);
   }
 }
 
 void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_size, const int* work, const int* copies,
-                long long max_copies, int* table, long long entries, const int* page_map, int pages, int num_sms,
-                cudaStream_t s) {
-  bool wide = true;
+                long long max_copies, int* table, long long entries, const int* page_map, int pages, int* err,
+                int num_sms, cudaStream_t s) {
   auto plane = [&](const PagePlane& p) {
-    CopyPlane c = {static_cast<char*>(p.base), p.layer_stride, p.token_bytes * block_size, p.token_bytes, 0};
-    if (p.base && ((reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.layer_stride | (uintptr_t)c.page_bytes) & 15)) wide = false;
-    return c;
+    return CopyPlane{static_cast<char*>(p.base), p.layer_stride, p.token_bytes * block_size, p.token_bytes};
   };
-  CopyPlane ca = plane(a), cb = plane(b);
-  const int vec = wide ? 16 : 4;
-  for (CopyPlane* c : {&ca, &cb}) c->pieces = c->base ? (c->page_bytes / vec + kPiece - 1) / kPiece : 0;
-  const long long units = max_copies * layers * (ca.pieces + cb.pieces);
-  const long long remap = (entries + kCopyThreads - 1) / kCopyThreads;
-  const long long want = std::max(units, table ? remap : 0ll);
+  const CopyPlane ca = plane(a), cb = plane(b);
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.base) | (uintptr_t)a.layer_stride | (uintptr_t)ca.page_bytes) & 15) == 0;
+  // pieces of about equal size: a 73,728-byte page in three of a whole stage
+  const int pieces = wide ? (ca.page_bytes + kStageBytes - 1) / kStageBytes : 1;
+  const int piece_bytes = ((ca.page_bytes + pieces - 1) / pieces + 15) / 16 * 16;
+  const long long units = max_copies * layers * pieces;
+  if (units >= (1ll << 30)) throw std::runtime_error("pages: too many pieces to copy in one call");
+  const long long want = std::max(units, table ? (entries + kCopyThreads - 1) / kCopyThreads : 0ll);
   if (want <= 0) return;
-  const int grid = (int)std::min<long long>(want, 8ll * num_sms);
-  if (wide) launch_k(pages_copy_kernel<uint4>, dim3(grid), dim3(kCopyThreads), 0, s, work, copies, layers, ca, cb, table,
-                     entries, page_map, pages);
-  else launch_k(pages_copy_kernel<int>, dim3(grid), dim3(kCopyThreads), 0, s, work, copies, layers, ca, cb, table,
-                entries, page_map, pages);
+  if (wide) {
+    set_smem_bytes(pages_copy_kernel, kStages * kStageBytes);
+    launch_k(pages_copy_kernel, dim3((unsigned)std::min<long long>(want, (long long)kCopyCtas * num_sms)),
+             dim3(kCopyThreads), kStages * kStageBytes, s, work, copies, layers, ca, cb, pieces, piece_bytes, table,
+             entries, page_map, pages, err);
+  } else {
+    launch_k(pages_copy_words_kernel, dim3((unsigned)std::min<long long>(want, 8ll * num_sms)), dim3(kCopyThreads), 0,
+             s, work, copies, layers, ca, cb, table, entries, page_map, pages);
+  }
 }
 
 }  // namespace sp

@@ -353,8 +353,8 @@ void pages_compact(int* refs, int pages, int block_size, int* page_map, int* liv
 void pages_pairs(const int* src, const int* dst, int n, int pages, int block_size, int* work, int* copies, int* err,
                  cudaStream_t s);
 void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_size, const int* work, const int* copies,
-                long long max_copies, int* table, long long entries, const int* page_map, int pages, int num_sms,
-                cudaStream_t s);
+                long long max_copies, int* table, long long entries, const int* page_map, int pages, int* err,
+                int num_sms, cudaStream_t s);
 // Phase clocks: totals[slot] += now - stamps[prev] (prev >= 0); stamps[slot] <- device global timer (ns).
 void phase_mark(unsigned long long* stamps, unsigned long long* totals, int slot, int prev, cudaStream_t s);
 void decode_advance(const int* out_ids, int* ids, int* pos, int* ctx, int* slots, const int* block_table,

@@ -58,6 +58,7 @@ struct Lm {
 struct LmParams {
   int T, V, K;
   int row_tiles, units, shares;  // row tiles, units of the vocabulary, shares of a row tile
+  int x_bytes;                   // of a box of x: one row tile loads only the rows that there are
   const int* ids;
   float4* part;                  // [shares * 2][row_tiles * 128]: m, S, E (log2 units), the given token's logit
   int* err;
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
               break;
             }
             uint8_t* at = smem + s * kStageBytes;
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (kXBytes + n * kBoxBytes));
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (p.x_bytes + n * kBoxBytes));
             if (CTAS == 2) {
               const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
               tma_load_2d_pair(at, &tmX, bar, kb * kBlockK, row);
@@ -295,25 +296,42 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
   }
 }
 
-// One warp per row joins its shares.
+// One warp per row joins its shares; a lane has all its parts under way before it uses one.
 __global__ void __launch_bounds__(128) lm_logprobs_join_kernel(const float4* __restrict__ part, int parts, int pitch,
                                                                int T, int V, const int* __restrict__ ids,
                                                                float* __restrict__ lp, float* __restrict__ entropy) {
+  constexpr int kAhead = 10;  // 320 parts at once: two for each of 148 CTAs
   griddep_wait();
   griddep_launch();
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= T) return;
+  const int id = ids[row];
   float m = -INFINITY, given = 0.f;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part[(long long)i * pitch + row].x);
-  m = warp_max(m);
   double s = 0.0, e = 0.0;
-  for (int i = lane; i < parts; i += 32) {
-    const float4 t = part[(long long)i * pitch + row];
-    const float d = t.x == -INFINITY ? 0.f : fmaxf((t.x - m) * kLog2e, -300.f);
-    const double f = fast_exp2(d);
-    s += f * t.y;
-    e += f * (t.z + t.y * d);
-    given += t.w;  // one share's, the others hold 0
+  for (int i0 = 0; i0 < parts; i0 += 32 * kAhead) {
+    float4 t[kAhead];
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * 32 + lane;
+      t[u] = i < parts ? part[(long long)i * pitch + row] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) top = fmaxf(top, t[u].x);
+    top = warp_max(top);
+    const float d0 = m == -INFINITY ? 0.f : fmaxf((m - top) * kLog2e, -300.f);
+    const double f0 = fast_exp2(d0);
+    e = f0 * (e + s * d0);
+    s = f0 * s;
+    m = top;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float d = t[u].x == -INFINITY ? 0.f : fmaxf((t[u].x - top) * kLog2e, -300.f);
+      const float f = fast_exp2(d);
+      s += f * t[u].y;
+      e += f * fmaf(t[u].y, d, t[u].z);
+      given += t[u].w;  // one share's, the others hold 0
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -324,7 +342,6 @@ __global__ void __launch_bounds__(128) lm_logprobs_join_kernel(const float4* __r
   if (lane != 0) return;
   const bool bad = s != s, empty = !bad && s == 0.0;
   const float log_s = empty ? 0.f : s < 2.0 ? log1pf(float(s - 1.0)) : logf(float(s));
-  const int id = ids[row];
   entropy[row] = bad ? NAN : empty ? 0.f : float(log_s - e / s * kLn2);
   lp[row] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (given - (empty ? 0.f : m)) - log_s;
 }
@@ -335,12 +352,15 @@ struct LmPlan {
   int ctas, row_tiles, units, shares;
 };
 
-// CTA pairs from two row tiles on. The vocabulary's shares per row tile are as many as leave
-// the busiest CTA the fewest units, counting an item's start as one more.
+// CTA pairs read half as much of w per SM, which lifts 8,192 x 102,400 x 2,048 from 2.83 to
+// 2.46 ms (1,400 TFLOP/s) and 512 rows from 195 to 174 us; below two tiles per SM the single
+// CTAs' finer items win (333 x 10,007 x 1,000: 20 against 24 us). The vocabulary's shares per
+// row tile are as many as leave the busiest CTA the fewest units, counting an item's start as
+// one more.
 LmPlan lm_plan(int T, int V, int num_sms) {
   LmPlan l;
-  l.ctas = T > kRows ? 2 : 1;
-  if (const char* e = getenv("LM_CTAS")) l.ctas = atoi(e);
+  const long long tiles = (long long)((T + kRows - 1) / kRows) * ((V + kCols - 1) / kCols);
+  l.ctas = T > kRows && tiles >= 2ll * num_sms ? 2 : 1;
   l.row_tiles = (T + kRows * l.ctas - 1) / (kRows * l.ctas);
   l.units = (V + kBox * l.ctas - 1) / (kBox * l.ctas);
   const int workers = num_sms / l.ctas;
@@ -406,8 +426,13 @@ void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int
   p.ids = ids;
   p.part = static_cast<float4*>(workspace);
   p.err = err;
+  // A few rows load only themselves (in swizzle atoms of 8): a CTA's copies move about 55 GB/s
+  // in rows of 128 bytes, and x, read again for each tile, should not take a third of it. The
+  // MMA's other rows are whatever shared memory held; theirs are results that nobody reads.
+  const int x_rows = l.row_tiles * l.ctas == 1 ? (T + 7) / 8 * 8 : kRows;
+  p.x_bytes = x_rows * kBlockK * 2;
   CUtensorMap tx, tw;
-  make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, kRows, kBlockK);
+  make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows, kBlockK);
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
   if (l.ctas == 2) launch_lm<2>(l, tx, tw, p, num_sms, s);
   else launch_lm<1>(l, tx, tw, p, num_sms, s);

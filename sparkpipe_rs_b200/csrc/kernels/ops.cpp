@@ -1196,42 +1196,39 @@ int64_t copy_pages(const Tensor& data, const c10::optional<Tensor>& scales, cons
   const int64_t n = src.numel();
   if (n == 0 || data.numel() == 0) return 0;
   const c10::cuda::CUDAGuard guard(data.device());
-  const Tensor work = torch::empty({3 * n + 1}, src.options());
+  const Tensor work = at::empty({3 * n + 1}, src.options());
   int* w = work.data_ptr<int>();
   sp::pages_pairs(src.data_ptr<int>(), dst.data_ptr<int>(), (int)n, (int)pages, (int)block_size, w + 1, w, err_word(),
                   stream());
   sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, std::min(n, pages), nullptr, 0, nullptr, 0,
-                 num_sms(), stream());
+                 err_word(), num_sms(), stream());
   return 2;
 }
 
-int64_t fork_pages(const Tensor& table, const Tensor& lens, const Tensor& parents, const Tensor& refs,
-                   int64_t block_size, const Tensor& new_table, const Tensor& new_lens) {
+std::tuple<Tensor, Tensor> fork_pages(const Tensor& table, const Tensor& lens, const Tensor& parents,
+                                      const Tensor& refs, int64_t block_size) {
   check_page_table(table, refs, "fork_pages");
-  check_page_table(new_table, refs, "fork_pages");
-  CHECK_I32(lens); CHECK_CONTIG(lens); CHECK_I32(parents); CHECK_CONTIG(parents); CHECK_I32(new_lens);
+  CHECK_I32(lens); CHECK_CONTIG(lens); CHECK_I32(parents); CHECK_CONTIG(parents);
   TORCH_CHECK(block_size >= 1 && block_size <= INT_MAX, "fork_pages: block_size");
   TORCH_CHECK(lens.dim() == 1 && lens.numel() == table.size(0), "fork_pages: one length per block_table row");
-  TORCH_CHECK(parents.dim() == 1 && new_table.size(0) == parents.numel() && new_table.size(1) == table.size(1) &&
-              new_lens.numel() == parents.numel(), "fork_pages: one parent per new row");
+  TORCH_CHECK(parents.dim() == 1 && parents.numel() <= INT_MAX / 2, "fork_pages: parents must be [n]");
   CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, parents); CHECK_ON(table, refs);
-  CHECK_ON(table, new_table); CHECK_ON(table, new_lens);
   const c10::cuda::CUDAGuard guard(table.device());
-  if (table.size(0) + parents.numel() == 0) return 0;
-  sp::pages_fork(table.data_ptr<int>(), (int)table.size(0), (int)table.size(1), lens.data_ptr<int>(),
-                 parents.data_ptr<int>(), (int)parents.numel(), refs.data_ptr<int>(), (int)refs.numel(),
-                 (int)block_size, new_table.data_ptr<int>(), new_lens.data_ptr<int>(), stream());
-  return 1;
+  const int64_t n = parents.numel(), cols = table.size(1);
+  const Tensor new_table = at::empty({n, cols}, table.options()), new_lens = at::empty({n}, table.options());
+  sp::pages_fork(table.data_ptr<int>(), (int)table.size(0), (int)cols, lens.data_ptr<int>(), parents.data_ptr<int>(),
+                 (int)n, refs.data_ptr<int>(), (int)refs.numel(), (int)block_size, new_table.data_ptr<int>(),
+                 new_lens.data_ptr<int>(), stream());
+  return {new_table, new_lens};
 }
 
-int64_t reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& data,
-                      const c10::optional<Tensor>& scales, const c10::optional<Tensor>& row_tokens, int64_t tokens,
-                      int64_t block_size, const Tensor& short_by) {
+Tensor reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& data,
+                     const c10::optional<Tensor>& scales, const c10::optional<Tensor>& row_tokens, int64_t tokens,
+                     int64_t block_size) {
   check_page_table(table, refs, "reserve_pages");
   const int64_t rows = table.size(0);
-  CHECK_I32(lens); CHECK_CONTIG(lens); CHECK_I32(short_by); CHECK_CONTIG(short_by);
-  TORCH_CHECK(lens.dim() == 1 && lens.numel() == rows && short_by.numel() == rows,
-              "reserve_pages: one length per block_table row");
+  CHECK_I32(lens); CHECK_CONTIG(lens);
+  TORCH_CHECK(lens.dim() == 1 && lens.numel() == rows, "reserve_pages: one length per block_table row");
   TORCH_CHECK(rows <= sp::kPagesMaxRows, "reserve_pages: at most " + std::to_string(sp::kPagesMaxRows) + " rows");
   TORCH_CHECK(tokens >= 0 && tokens <= INT_MAX, "reserve_pages: tokens must not be negative");
   sp::PagePlane a, b;
@@ -1242,19 +1239,19 @@ int64_t reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& ref
     TORCH_CHECK(row_tokens->dim() == 1 && row_tokens->numel() == rows, "reserve_pages: one token count per row");
     CHECK_ON(table, *row_tokens);
   }
-  CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, refs); CHECK_ON(table, data); CHECK_ON(table, short_by);
+  CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, refs); CHECK_ON(table, data);
   const c10::cuda::CUDAGuard guard(table.device());
-  if (rows == 0) return 0;
-  const Tensor work = torch::empty({1 + 3 * rows + refs.numel()}, table.options());
+  const Tensor short_by = at::empty({rows}, table.options());
+  if (rows == 0) return short_by;
+  const Tensor work = at::empty({1 + 3 * rows + refs.numel()}, table.options());
   int* w = work.data_ptr<int>();
   sp::pages_reserve(table.data_ptr<int>(), (int)rows, (int)table.size(1), lens.data_ptr<int>(),
                     row_tokens.has_value() ? row_tokens->data_ptr<int>() : nullptr, (int)tokens,
                     refs.data_ptr<int>(), (int)refs.numel(), (int)block_size, w + 1 + 3 * rows, w + 1, w,
                     short_by.data_ptr<int>(), stream());
-  if (data.numel() == 0) return 1;
   sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, std::min<int64_t>(rows, refs.numel()), nullptr, 0,
-                 nullptr, 0, num_sms(), stream());
-  return 2;
+                 nullptr, 0, err_word(), num_sms(), stream());
+  return short_by;
 }
 
 int64_t free_pages(const Tensor& table, const Tensor& refs, const c10::optional<Tensor>& rows) {
@@ -1273,24 +1270,23 @@ int64_t free_pages(const Tensor& table, const Tensor& refs, const c10::optional<
   return 1;
 }
 
-int64_t compact_pages(const Tensor& table, const Tensor& refs, const Tensor& data, const c10::optional<Tensor>& scales,
-                      int64_t block_size, const Tensor& page_map, const Tensor& live) {
+std::tuple<Tensor, Tensor> compact_pages(const Tensor& table, const Tensor& refs, const Tensor& data,
+                                         const c10::optional<Tensor>& scales, int64_t block_size) {
   check_page_table(table, refs, "compact_pages");
   sp::PagePlane a, b;
   const int64_t pages = page_planes(data, scales, block_size, &a, &b, "compact_pages");
   TORCH_CHECK(refs.numel() <= pages, "compact_pages: refs counts more pages than the cache has");
-  CHECK_I32(page_map); CHECK_CONTIG(page_map); CHECK_I32(live);
-  TORCH_CHECK(page_map.numel() == refs.numel() && live.numel() == 1, "compact_pages: output shapes");
-  CHECK_CUDA(table); CHECK_ON(table, refs); CHECK_ON(table, data); CHECK_ON(table, page_map); CHECK_ON(table, live);
+  CHECK_CUDA(table); CHECK_ON(table, refs); CHECK_ON(table, data);
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t n = refs.numel();
-  const Tensor work = torch::empty({1 + 4 * n}, table.options());
+  const Tensor page_map = at::empty({n}, refs.options()), live = at::empty({1}, refs.options());
+  const Tensor work = at::empty({1 + 4 * n}, table.options());
   int* w = work.data_ptr<int>();
   sp::pages_compact(refs.data_ptr<int>(), (int)n, (int)block_size, page_map.data_ptr<int>(), live.data_ptr<int>(),
                     w + 1, w + 1 + 3 * n, w, stream());
   sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, n / 2, table.data_ptr<int>(), table.numel(),
-                 page_map.data_ptr<int>(), (int)n, num_sms(), stream());
-  return 2;
+                 page_map.data_ptr<int>(), (int)n, err_word(), num_sms(), stream());
+  return {page_map, live};
 }
 
 }  // namespace

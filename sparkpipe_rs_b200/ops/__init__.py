@@ -659,11 +659,9 @@ def fork_pages(block_table, lens, parents, refs, block_size=64):
     them, are given up: refs changes by what the new rows hold less what the old ones held.
     No page is copied; ``reserve_pages`` makes a shared last page private before it is
     written."""
-    n = parents.shape[0]
-    table = torch.empty(n, block_table.shape[1], dtype=torch.int32, device=block_table.device)
-    new_lens = torch.empty(n, dtype=torch.int32, device=block_table.device)
-    _count(kernels().fork_pages(block_table, lens, parents, refs, int(block_size), table, new_lens))
-    return table, new_lens
+    out = kernels().fork_pages(block_table, lens, parents, refs, int(block_size))
+    _count(1 if block_table.shape[0] + parents.shape[0] else 0)
+    return out
 
 
 def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, cache_scales=None):
@@ -675,10 +673,10 @@ def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, 
     Rows are served in order, each wholly or not at all; returns int32 [rows], the pages that
     a row lacks (0: it may be written). The table's width bounds a row. At most
     PAGES_MAX_ROWS rows."""
-    short = torch.empty(block_table.shape[0], dtype=torch.int32, device=block_table.device)
     per_row = tokens if isinstance(tokens, torch.Tensor) else None
-    _count(kernels().reserve_pages(block_table, lens, refs, cache_data, cache_scales, per_row,
-                                   0 if per_row is not None else int(tokens), int(block_size), short))
+    short = kernels().reserve_pages(block_table, lens, refs, cache_data, cache_scales, per_row,
+                                    0 if per_row is not None else int(tokens), int(block_size))
+    _count((1 + (cache_data.numel() > 0)) if block_table.shape[0] else 0)
     return short
 
 
@@ -693,10 +691,9 @@ def compact_pages(block_table, refs, cache_data, block_size=64, cache_scales=Non
     the j-th live page at or behind L moves to the j-th free page before L, in every layer;
     block_table and refs follow. Returns (page_map [pages] int32: each page's new place, -1
     for a free one, for whatever else holds pages; L as int32 [1])."""
-    page_map = torch.empty(refs.shape[0], dtype=torch.int32, device=refs.device)
-    live = torch.empty(1, dtype=torch.int32, device=refs.device)
-    _count(kernels().compact_pages(block_table, refs, cache_data, cache_scales, int(block_size), page_map, live))
-    return page_map, live
+    out = kernels().compact_pages(block_table, refs, cache_data, cache_scales, int(block_size))
+    _count(2)
+    return out
 
 
 def gather_prev_tokens(ids, prev, n):
