@@ -51,6 +51,9 @@ class ForwardBatch:
     max_q: int = 0
     ctx_slots: torch.Tensor | None = None     # [Tk] cache rows of every context token (prefix + chunk)
     logits_idx: torch.Tensor | None = None    # rows to compute logits for (None = all)
+    # the token that follows each of those rows (-1: none): forward then returns their log
+    # probabilities and the rows' entropy instead of logits, which are never stored
+    score_ids: torch.Tensor | None = None
 
 
 class PhaseClock:
@@ -469,7 +472,8 @@ class MLAMoEModel:
     def forward(self, fb: ForwardBatch, cache: KVCache, layers: range | None = None,
                 hidden_in: torch.Tensor | None = None, return_hidden: bool = False, layer_offset: int = 0):
         """Runs `layers` (default: all) and returns logits [n, V] (bf16) of the rows in
-        fb.logits_idx, or the residual stream when return_hidden (pipeline stages).
+        fb.logits_idx (with fb.score_ids: (logprobs [n], entropy [n]) of those tokens), or
+        the residual stream when return_hidden (pipeline stages).
         Model layer i uses cache layer i - layer_offset (a stage caches only its layers)."""
         self._layer_offset = layer_offset
         c, w = self.cfg, self.w
@@ -516,7 +520,10 @@ class MLAMoEModel:
         if self.ep is not None:
             self.ep.end_step()
         sel = xn if fb.logits_idx is None else ops.gather_rows(xn, fb.logits_idx)
-        logits = ops.linear(sel, w["lm_head"])
+        if fb.score_ids is not None:
+            logits = ops.linear_logprobs(sel, w["lm_head"], fb.score_ids)
+        else:
+            logits = ops.linear(sel, w["lm_head"])
         if pc is not None:
             pc.mark(4, prev)
         return logits
@@ -526,14 +533,18 @@ class DecodeGraph:
     """One CUDA graph of a full decode step (forward + sampling) for a fixed batch
     size. Inputs are copied into static device buffers before replay; sampling reads
     a per-row temperature and noise key (``temps`` / ``keys``, zero = greedy), so one
-    graph serves greedy and sampled requests in the same batch."""
+    graph serves greedy and sampled requests in the same batch. With ``logprobs`` >= 0 the
+    step also leaves ``scores``, the sampled tokens' log probabilities with that many
+    alternatives (``ops.TokenLogprobs`` of the logits before temperature)."""
 
     def __init__(self, model: MLAMoEModel, cache: KVCache, batch: int, max_blocks: int, max_context: int,
-                 use_graph: bool = True, self_advance: bool = False, extra=None):
+                 use_graph: bool = True, self_advance: bool = False, extra=None, logprobs: int = -1):
         """``extra(fb)``: more device work of the step, captured into the same graph
         (the serving engine keeps a draft model's KV current with it)."""
         self.model, self.cache, self.B = model, cache, batch
         self.extra = extra
+        self.logprobs = logprobs
+        self.scores = None
         dev = model.device
         self.ids = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
@@ -568,6 +579,8 @@ class DecodeGraph:
     def _step(self):
         logits = self.model.forward(self.fb, self.cache)
         ops.sample_tokens(logits, out_ids=self.out_ids, row_temp=self.temps, row_key=self.keys)
+        if self.logprobs >= 0:
+            self.scores = ops.token_logprobs(logits, self.out_ids, top_k=self.logprobs)
         if self.extra is not None:
             self.extra(self.fb)
         if self.self_advance:
@@ -585,4 +598,4 @@ class DecodeGraph:
         return self.out_ids
 
     def release(self):
-        self.graph = None
+        self.graph = self.scores = None

@@ -87,6 +87,7 @@ class EngineConfig:
     host_drive_path: str = ""         # with fewer resident buffers than slots: the drive file the rest spill to
     kv_cache_dtype: str = "bf16"      # "fp8": e4m3 latent rows with per-128 block scales (CUDA, 576-wide rows)
     warm_prefill: bool = True         # one throwaway prefill of the largest chunk at start (allocator warm-up)
+    logprobs: int = -1                # >= 0: log probability of every generated token, with that many alternatives
     prefill_graphs: bool = False      # replay repeated prefill chunk shapes (no cached prefix) from CUDA graphs
 
 
@@ -110,6 +111,10 @@ class RequestOutput:
     arrival: float = 0.0
     first_token_time: float = 0.0
     finish_time: float = 0.0
+    # with EngineConfig.logprobs >= 0, one entry per generated token
+    logprobs: list = field(default_factory=list)
+    entropies: list = field(default_factory=list)       # of the distribution before temperature
+    top_logprobs: list = field(default_factory=list)    # [(token id, log probability)], most probable first
 
     @property
     def ttft(self) -> float:
@@ -192,6 +197,7 @@ class _Launched:
     out: torch.Tensor      # device tensor of the sampled tokens
     t0: float
     timing: tuple | None = None  # CUDA events around the step's device work (cost model)
+    scores: list | None = None   # host tensors of the tokens' log probabilities (EngineConfig.logprobs)
 
 
 class _PrefillGraph:
@@ -244,6 +250,12 @@ class LLMEngine:
         if e.speculation not in ("", "chain", "mtp_tree"):
             raise ValueError(f"unknown speculation mode {e.speculation!r}")
         self.spec = e.speculation
+        if e.logprobs >= 0:
+            if not self.is_cuda or not isinstance(self.model, MLAMoEModel) or self.spec:
+                raise ValueError("logprobs need the GPU model without speculation")
+            if e.logprobs > min(ops.kernels().LOGPROBS_MAX_TOP, cfg.vocab_size):
+                raise ValueError(f"logprobs: at most {ops.kernels().LOGPROBS_MAX_TOP} alternatives")
+        self._scores = None
         buckets = [b for b in e.decode_buckets if b <= max(e.max_batch, 1)] + (
             [e.max_batch] if e.max_batch not in e.decode_buckets else [])
         # tree verify: two shadow KV rows per batch row, past the scheduler's blocks
@@ -402,11 +414,15 @@ class LLMEngine:
         rows = self._sampling_rows(plan, logits.shape[0], "p")
         if self.is_cuda:
             if rows is None:
-                return ops.sample_tokens(logits)
-            temps, keys = rows
-            self.h2d_bytes += temps.numel() * 12
-            return ops.sample_tokens(logits, row_temp=temps.to(self.device, non_blocking=True),
-                                     row_key=keys.to(self.device, non_blocking=True))
+                out = ops.sample_tokens(logits)
+            else:
+                temps, keys = rows
+                self.h2d_bytes += temps.numel() * 12
+                out = ops.sample_tokens(logits, row_temp=temps.to(self.device, non_blocking=True),
+                                        row_key=keys.to(self.device, non_blocking=True))
+            if self.ecfg.logprobs >= 0:
+                self._scores = ops.token_logprobs(logits, out, top_k=self.ecfg.logprobs)
+            return out
         out = logits.float().argmax(-1).to(torch.int32)
         if rows is not None:  # Gumbel-max per sampled row, noise seeded by the row's key
             temps, keys = rows
@@ -421,7 +437,8 @@ class LLMEngine:
         g = self.graphs.get(bucket)
         if g is None:
             g = DecodeGraph(self.model, self.cache, bucket, self.max_blocks, self.ecfg.max_model_len,
-                            use_graph=self.ecfg.use_cuda_graph, extra=self._draft_kv if self.spec else None)
+                            use_graph=self.ecfg.use_cuda_graph, extra=self._draft_kv if self.spec else None,
+                            logprobs=self.ecfg.logprobs)
             self.graphs[bucket] = g
         return g
 
@@ -614,11 +631,14 @@ class LLMEngine:
             out = g.run()
             self._timing[1].record()
             return out
-        return g.run()
+        out = g.run()
+        self._scores = g.scores
+        return out
 
     def _launch(self, plan, prev: _Launched | None = None) -> _Launched:
         t0 = time.perf_counter()
-        self._timing = None
+        self._timing = self._scores = None
+        scores = None
         try:
             if plan.kind == 3:
                 return self._launch_verify(plan, t0)
@@ -633,6 +653,13 @@ class LLMEngine:
             if self.is_cuda:
                 host = self.pinned.get(f"sampled{self._parity}", n)
                 host.copy_(sampled[:n], non_blocking=True)
+                if self._scores is not None:
+                    scores = []
+                    for name, t in zip(("lp", "ent", "tlp", "tid"), self._scores):
+                        buf = self.pinned.get(f"{name}{self._parity}", t[:n].numel(), t.dtype).view(t[:n].shape)
+                        buf.copy_(t[:n], non_blocking=True)
+                        scores.append(buf)
+                        self.d2h_bytes += buf.numel() * 4
                 ev = torch.cuda.Event()
                 ev.record()
                 self.d2h_bytes += n * 4
@@ -641,7 +668,7 @@ class LLMEngine:
         except Exception:
             self.scheduler.fail_step(plan)
             raise
-        return _Launched(plan, host, ev, sampled, t0, self._timing)
+        return _Launched(plan, host, ev, sampled, t0, self._timing, scores)
 
     def _launch_verify(self, plan, t0: float) -> _Launched:
         committed, counts, paths = self._run_verify(plan)
@@ -781,6 +808,7 @@ class LLMEngine:
             self.step_log.append(("prefill" if plan.kind == 1 else "decode", plan.num_seqs, dt, plan.num_tokens))
             events = self.scheduler.complete_tensor(plan, cur.host)
         changed = {}
+        rows = {int(q): i for i, q in enumerate(plan.seq_ids)} if cur.scores is not None else None
         for ev in events:
             out = self.outputs.get(ev.id)
             if out is None:
@@ -789,6 +817,11 @@ class LLMEngine:
                 if not out.token_ids:
                     out.first_token_time = now
                 out.token_ids.append(int(ev.token))
+                if rows is not None:
+                    lp, ent, top_lp, top_ids = (t[rows[int(ev.id)]] for t in cur.scores)
+                    out.logprobs.append(float(lp))
+                    out.entropies.append(float(ent))
+                    out.top_logprobs.append(list(zip(top_ids.tolist(), top_lp.tolist())))
                 changed[ev.id] = out
             elif ev.kind == 2:  # finished
                 out.finished = True
@@ -799,6 +832,43 @@ class LLMEngine:
         return changed
 
     # ------------------------------------------------------------------ batch API
+    def score(self, prompts) -> list[list[float]]:
+        """Log probability of every prompt token but the first, given the tokens before it:
+        one list per prompt, one shorter than it. Prompts run whole, several to a forward of
+        at most ``max_prefill_tokens`` tokens; nothing is cached and no logits are stored."""
+        if not self.is_cuda or not isinstance(self.model, MLAMoEModel) or self._lockstep is not None:
+            raise ValueError("score needs the GPU model on one rank")
+        limit = self.ecfg.max_prefill_tokens
+        out: list[list[float]] = [[] for _ in prompts]
+        todo = []
+        for i, p in enumerate(prompts):
+            if len(p) > min(limit, self.ecfg.max_model_len):
+                raise ValueError(f"score: a prompt of {len(p)} tokens exceeds one prefill chunk ({limit}) or the model length")
+            if not all(0 <= int(t) < self.cfg.vocab_size for t in p):
+                raise ValueError("score: token ids outside the vocabulary")
+            if len(p) > 1:
+                todo.append(i)
+        i32 = dict(dtype=torch.int32, device=self.device)
+        while todo:
+            batch, tokens = [], 0
+            while todo and tokens + len(prompts[todo[0]]) <= limit:
+                batch.append(todo.pop(0))
+                tokens += len(prompts[batch[-1]])
+            lens = [len(prompts[i]) for i in batch]
+            ids = [int(t) for i in batch for t in prompts[i]]
+            nxt = [int(t) for i in batch for t in list(prompts[i][1:]) + [-1]]
+            cu = torch.tensor([0] + list(itertools.accumulate(lens)), **i32)
+            fb = ForwardBatch(mode="prefill", token_ids=torch.tensor(ids, **i32),
+                              positions=torch.tensor([t for n in lens for t in range(n)], **i32),
+                              slot_mapping=torch.full((tokens,), -1, **i32), cu_q=cu, cu_k=cu, max_q=max(lens),
+                              score_ids=torch.tensor(nxt, **i32))
+            lp = self.model.forward(fb, self.cache)[0].tolist()
+            at = 0
+            for i, n in zip(batch, lens):
+                out[i] = lp[at:at + n - 1]
+                at += n
+        return out
+
     def generate(self, prompts, params: SamplingParams | None = None) -> GenerateResult:
         """Submits every prompt, runs steps until all finish; returns outputs and serving stats."""
         params = params or SamplingParams()
