@@ -43,8 +43,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-// 64 registers: with 48 the loop spills, with 80 fewer warps hide the exponentials (8,192 rows x
-// 102,400 without alternatives: 296 us, against 314 at five CTAs and 322 at three)
+// 64 registers, which hold a batch and the next one's loads (8,192 rows x 102,400 with 20
+// alternatives: 323 us, 346 us without the loads ahead; with 80 registers 342 us, with 48 and
+// half as large batches 336 us)
 constexpr int kCtasPerSm = 4;
 constexpr int kBatch = 4;         // 16-byte vectors of a batch, in flight together
 constexpr int kSlots = 16;        // recorded batch maxima of a thread (several batches each in longer rows)
@@ -297,48 +298,69 @@ SP_DEVI void join_stats(const Shared& sh, int n, float& m, double& s, double& e)
 }
 
 // More logits reach the floor than the list holds: each thread offers its best one not
-// yet taken, the CTA takes the best of these, k times.
+// yet taken, the CTA takes the best of these, k times. The next offer of the thread whose
+// one was taken is found by its whole warp.
 template <typename T>
 __device__ __noinline__ void pick_rounds(const Part<T>& part, int nb, int k, Shared& sh) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  float pv = INFINITY, best = -INFINITY;
-  int pi = -1, at = kNone;
-  bool scan = true;
-  for (int r = 0; r < k; ++r) {
-    if (scan) {
-      best = -INFINITY;
-      at = kNone;
-      auto see = [&](float v, int i) {
-        if (v != -INFINITY && i >= 0 && before(pv, pi, v, i) && before(v, i, best, at)) { best = v; at = i; }
-      };
-      part.batches(0, nb, see);
-      part.singles(see);
-    }
-    float bv = best;
-    int bi = at;
+  float best = -INFINITY;
+  int at = kNone;
+  auto first_of_warp = [](float& v, int& i) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+      const float ov = __shfl_xor_sync(0xffffffffu, v, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, i, o);
+      if (before(ov, oi, v, i)) { v = ov; i = oi; }
     }
+  };
+  auto offer = [&](float v, int i) {
+    if (v != -INFINITY && i >= 0 && before(v, i, best, at)) { best = v; at = i; }
+  };
+  part.batches(0, nb, offer);
+  part.singles(offer);
+  for (int r = 0; r < k; ++r) {
+    float pv = best;
+    int pi = at;
+    first_of_warp(pv, pi);
     __syncthreads();
     if (lane == 0) {
-      sh.v[w] = bv;
-      sh.id[w] = bi;
+      sh.v[w] = pv;
+      sh.id[w] = pi;
     }
     __syncthreads();
     for (int i = 0; i < kWarps; ++i)
-      if (before(sh.v[i], sh.id[i], bv, bi)) { bv = sh.v[i]; bi = sh.id[i]; }
+      if (before(sh.v[i], sh.id[i], pv, pi)) { pv = sh.v[i]; pi = sh.id[i]; }
+    if (pi == kNone) break;  // the same for every thread
     if (threadIdx.x == 0) {
-      sh.v[kWarps + r] = bv;
-      sh.id[kWarps + r] = bi;
-      if (bi != kNone) sh.n = r + 1;
+      sh.v[kWarps + r] = pv;
+      sh.id[kWarps + r] = pi;
+      sh.n = r + 1;
     }
-    pv = bv;
-    pi = bi;
-    scan = bi != kNone && bi == at;  // this thread's offer was taken
-    if (bi == kNone) break;
+    const unsigned taken = __ballot_sync(0xffffffffu, at == pi);
+    if (taken) {  // this warp's thread `from`: its best logit that ranks after the one taken
+      const int from = __ffs(taken) - 1;
+      float nv = -INFINITY;
+      int ni = kNone;
+      auto next = [&](float v, int i) {
+        if (v != -INFINITY && i >= 0 && before(pv, pi, v, i) && before(v, i, nv, ni)) { nv = v; ni = i; }
+      };
+      for (int v = part.v0 + w * 32 + from + lane * kThreads; v < part.v1; v += 32 * kThreads) {
+        const uint4 q = __ldg(part.body + v);
+#pragma unroll
+        for (int j = 0; j < Logits<T>::N / 2; ++j) {
+          float x, y;
+          values2<T>(q, j, x, y);
+          next(x, part.first + v * Logits<T>::N + 2 * j);
+          next(y, part.first + v * Logits<T>::N + 2 * j + 1);
+        }
+      }
+      if (lane == from) part.singles(next);
+      first_of_warp(nv, ni);
+      if (lane == from) {
+        best = nv;
+        at = ni;
+      }
+    }
   }
   __syncthreads();
 }
@@ -402,20 +424,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   };
   const int whole = (part.v1 - part.v0) / (kBatch * kThreads);
   const uint4* src = part.body + part.v0 + threadIdx.x;
+  // the next batch's loads go out before this one's arithmetic
+  uint4 nx[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) nx[i] = part.vector(part.v0 + i * kThreads + threadIdx.x);
 #pragma unroll 1
   for (int b = 0; b < whole; ++b) {
     uint4 v[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) v[i] = __ldg(src + i * kThreads);
+    for (int i = 0; i < kBatch; ++i) v[i] = nx[i];
     src += kBatch * kThreads;
-    take(v);
-  }
-  if (whole < nb) {
-    uint4 v[kBatch];
+    if (b + 1 < whole) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) v[i] = part.vector(part.v0 + (whole * kBatch + i) * kThreads + threadIdx.x);
+      for (int i = 0; i < kBatch; ++i) nx[i] = __ldg(src + i * kThreads);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) nx[i] = part.vector(part.v0 + (whole * kBatch + i) * kThreads + threadIdx.x);
+    }
     take(v);
   }
+  if (whole < nb) take(nx);
   if (TOP && per_slot > 1 && left != per_slot) sh.slot[slot++][threadIdx.x] = slot_max;
   const float one = part.single(part.head), two = part.single(part.tail);
   if (part.head >= 0 || part.tail >= 0) {
