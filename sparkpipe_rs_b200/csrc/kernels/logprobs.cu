@@ -15,13 +15,14 @@
 //
 // What bounds it: one read of the logits. At 8,192 rows x 102,400 bf16 an SM takes in 11
 // logits per clock, which leaves room for about eleven instructions and one exponential
-// (16 per clock) for each, so the loop works on packed pairs. The alternatives cost one
-// comparison per batch: while it streams, a thread notes the maximum of each batch of 16
-// or 32 logits in shared memory. Of the 64 maxima of four threads each, the k-th largest
-// is a floor under the row's k-th largest logit; afterwards only batches whose maximum
-// reaches it are read again (about k of them), and the logits at or above the floor are
-// ranked by counting. Should ties leave more of them than the list holds, k rounds of
-// the CTA's maximum pick them one by one.
+// (16 per clock) for each, so the loop works on packed pairs: 6.8 instructions per logit, the
+// exponentials' pipe four fifths busy, 300 us (5.6 TB/s). The alternatives cost one comparison
+// per batch: while it streams, a thread notes the maximum of each batch of 16 or 32 logits in
+// shared memory. Of the 64 maxima of four threads each, the k-th largest is a floor under the
+// row's k-th largest logit; afterwards only batches whose maximum reaches it are read again
+// (about k of them), and the logits at or above the floor are ranked by counting: 325 us with
+// 20 alternatives. Should ties leave more of them than the list holds, k rounds of the CTA's
+// maximum pick them one by one (1.2 ms for 8,192 rows of equal logits).
 //
 // Few rows are split over the CTAs of a thread-block cluster, which join their sums and
 // lists through distributed shared memory: one launch, no workspace, nothing that two
@@ -76,6 +77,7 @@ struct Logits<__nv_bfloat16> {
   static constexpr unsigned kNegInf = 0xff80ff80u;
   // logits below `kLow` (-1e30) weigh nothing beside a maximum within (kMin, kMax)
   static constexpr float kMin = -1e29f, kMax = 1e29f;
+  static SP_DEVI unsigned max_nan2(unsigned a, unsigned b) { return max_nan_bf16x2(a, b); }
   static SP_DEVI unsigned raise(unsigned w) { return max_nan_bf16x2(w, 0xf149f149u); }
   static SP_DEVI float value(__nv_bfloat16 v) { return __bfloat162float(v); }
   static SP_DEVI void pair(unsigned w, float& a, float& b) {
@@ -92,6 +94,7 @@ struct Logits<__half> {
   static constexpr int N = 8;
   static constexpr unsigned kNegInf = 0xfc00fc00u;
   static constexpr float kMin = -60000.f, kMax = 65504.f * 2;  // raised to the type's lowest value, -65504
+  static SP_DEVI unsigned max_nan2(unsigned a, unsigned b) { return max_nan_f16x2(a, b); }
   static SP_DEVI unsigned raise(unsigned w) { return max_nan_f16x2(w, 0xfbfffbffu); }
   static SP_DEVI float value(__half v) { return __half2float(v); }
   static SP_DEVI void pair(unsigned w, float& a, float& b) {
@@ -109,6 +112,9 @@ struct Logits<float> {
   static constexpr int N = 4;
   static constexpr unsigned kNegInf = 0xff800000u;
   static constexpr float kMin = -1e29f, kMax = 1e29f;
+  static SP_DEVI unsigned max_nan2(unsigned a, unsigned b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
   static SP_DEVI unsigned raise(unsigned w) { return __float_as_uint(max_nan(__uint_as_float(w), -1e30f)); }
   static SP_DEVI float value(float v) { return v; }
   static SP_DEVI void pair(unsigned, float&, float&) {}
@@ -139,6 +145,17 @@ SP_DEVI float batch_max(const uint4 (&v)[kBatch]) {
   float a, b;
   L::pair(m, a, b);
   return fmaxf(a, b);
+}
+
+// Whether a batch is all -inf (no NaN either).
+template <typename T>
+SP_DEVI bool all_masked(const uint4 (&v)[kBatch]) {
+  using L = Logits<T>;
+  unsigned m = L::kNegInf;
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    m = L::max_nan2(m, L::max_nan2(L::max_nan2(v[i].x, v[i].y), L::max_nan2(v[i].z, v[i].w)));
+  return m == L::kNegInf;
 }
 
 // The sums of a batch's terms. Beside a maximum of ordinary size (CLAMP false) very small
@@ -182,8 +199,10 @@ __device__ __noinline__ float2 rare_terms(Batch b, float shift) {
 // (v, i) ranks before (w, j): larger logit, then lower id
 SP_DEVI bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
-// This CTA's part of a row: single logits before the first 16-byte boundary and behind the
-// last whole vector (at most one each per thread), vectors in between.
+// This CTA's part of a row: single logits before the first 128-byte line and behind the last
+// whole vector (at most one each per thread), vectors in between. Vectors that start with a
+// line let a warp's load touch four lines, not five: 515 rows x 129,281 fp32 went from 64 to
+// 57 us (129,280, whose rows all start with a line: 52 us).
 template <typename T>
 struct Part {
   const T* row;
@@ -194,12 +213,12 @@ struct Part {
 
   SP_DEVI Part(const T* r, int V, int rank, int parts) : row(r) {
     constexpr int N = Logits<T>::N;
-    const int skip = int((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / (int)sizeof(T);
+    const int skip = int((128 - (reinterpret_cast<uintptr_t>(r) & 127)) & 127) / (int)sizeof(T);
     first = min(skip, V);
     body = reinterpret_cast<const uint4*>(r + first);
     const int nv = (V - first) / N;
-    v0 = int((long long)nv * rank / parts);
-    v1 = int((long long)nv * (rank + 1) / parts);
+    v0 = int((long long)nv * rank / parts) & ~7;
+    v1 = rank == parts - 1 ? nv : int((long long)nv * (rank + 1) / parts) & ~7;
     const int t = threadIdx.x;
     head = rank == 0 && t < first ? t : -1;
     const int behind = first + nv * N;
@@ -402,6 +421,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     float bs, be;
     if (a.m > Logits<T>::kMin && a.m < Logits<T>::kMax) {
       batch_terms<T, false>(v, -a.m, bs, be);
+    } else if (a.m == -INFINITY && all_masked<T>(v)) {
+      bs = be = 0.f;  // a mask so far, which costs one maximum
     } else {
       Batch copy;
 #pragma unroll
@@ -654,8 +675,8 @@ static void dispatch(const T* logits, long long ld, int rows, int V, const int* 
                      float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
   // CTAs per row: few rows are split as long as that gives each SM two CTAs at most and each
   // CTA a whole batch. Split further, a row's join costs more than its stream gains: 64 rows x
-  // 102,400 bf16 with 20 alternatives take 16.8 us unsplit, 10.5 us in four, 11.0 us in eight;
-  // 515 rows 29.9 us unsplit, 38.0 us in two; one row 12.0 us unsplit, 6.5 us in eight.
+  // 102,400 bf16 with 20 alternatives take 9.7 us in four, 11.1 us in eight; 515 rows 29.9 us
+  // unsplit, 35.1 us in two; one row 7.4 us in four, 6.6 us in eight.
   const int batch = kBatch * kThreads * Logits<T>::N;
   int parts = 1;
   while (parts < kMaxCluster && (long long)rows * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= batch) parts *= 2;

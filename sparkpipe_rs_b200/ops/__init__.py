@@ -689,7 +689,7 @@ def free_pages(block_table, refs, rows=None):
 def compact_pages(block_table, refs, cache_data, block_size=64, cache_scales=None):
     """Moves the live pages (refs > 0) to the front of the cache, in place: with L of them,
     the j-th live page at or behind L moves to the j-th free page before L, in every layer;
-    block_table and refs follow. Returns (page_map [pages] int32: each page's new place, -1
+    block_table and refs follow (an entry that names a free page becomes -1). Returns (page_map [pages] int32: each page's new place, -1
     for a free one, for whatever else holds pages; L as int32 [1])."""
     out = kernels().compact_pages(block_table, refs, cache_data, cache_scales, int(block_size))
     _count(2)

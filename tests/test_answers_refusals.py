@@ -40,6 +40,15 @@ def _bf(*shape):
 @pytest.mark.parametrize("x,w,ids,says", [
     (_bf(4, 16), _bf(9, 16), i32(3), "one per row"),
     (_bf(4, 16), _bf(9, 16), i32(4, 1), "one per row"),
+    (_bf(4, 12), _bf(9, 12), i32(4), "multiple of 8"),
+    (_bf(4, 16), _bf(9, 24), i32(4), "x .T, K. and w"),
+    (_bf(4, 16), _bf(0, 16), i32(4), "no columns"),
+    (_bf(4, 16).float(), _bf(9, 16), i32(4), "bf16"),
+    (_bf(4, 16), _bf(9, 16), torch.zeros(4, dtype=torch.int64), "int32"),
+    (_bf(4, 20)[:, :16], _bf(9, 16), i32(4), "16-byte aligned"),
+    (_bf(4, 24)[:, 1:17], _bf(9, 16), i32(4), "16-byte aligned"),
+    (_bf(1, 16).expand(4, 16), _bf(9, 16), i32(4), "16-byte aligned"),
+    (_bf(16, 4).t(), _bf(9, 16), i32(4), "row-major"),
     (_bf(4, 16), _bf(9, 16), i32(4), "CUDA"),
 ])
 def test_linear_logprobs(x, w, ids, says):
@@ -99,6 +108,7 @@ def test_free_and_compact():
     for rows, says in ((i32(2, 2), "rows must be"), (torch.zeros(2), "int32"), (i32(2), "CUDA"), (None, "CUDA")):
         with pytest.raises((ValueError, RuntimeError), match=says):
             ops.free_pages(i32(3, 4), i32(2), rows)
+    assert ops.kernels().LOGPROBS_MAX_TOP == 32 and ops.kernels().PAGES_MAX_ROWS == 4000
     for refs, says in ((i32(3), "more pages than the cache"), (i32(2), "CUDA")):
         with pytest.raises((ValueError, RuntimeError), match=says):
             ops.compact_pages(i32(3, 4), refs, CACHE)
