@@ -109,126 +109,104 @@ void pages_fork(const int* table, int rows, int cols, const int* lens, const int
 }
 
 // ------------------------------------------------------------------ reserve
-// One CTA. Phase 1: what each row needs, and its place among the needs of the rows before
-// it; phase 2: the lowest free pages, as many as are needed; phase 3: grants. The counts of up
-// to kNearRefs pages and up to kGrants granted pages stay in shared memory, so that a beam
-// step pays two dependent reads of memory (a row's length, its last page); larger caches read
+// One CTA, a thread per row: what the row needs, its place among the needs of the rows before
+// it, the lowest free pages (as many as are needed), the grants. The counts of up to
+// kNearRefs pages and up to kGrants granted pages stay in shared memory, so that a beam step
+// pays two dependent reads of memory (a row's length, its last page); larger caches read
 // refs again, larger grants go through `free_list` [pages]. `work` gets the copy list, (source,
 // destination, tokens) records, and `copies` its length.
-__global__ void __launch_bounds__(kIndexThreads)
+__global__ void __launch_bounds__(kPagesMaxRows)
     pages_reserve_kernel(int* __restrict__ table, int rows, int cols, const int* __restrict__ lens,
                          const int* __restrict__ row_tokens, int tokens, int* refs, int pages, int block_size,
                          int* free_list, int* __restrict__ work, int* __restrict__ copies, int* __restrict__ short_by) {
   extern __shared__ int smem[];
-  int* tail = smem;             // [rows] last page if other rows hold it too, else -1
-  int* start = tail + rows;     // [rows] pages granted to the rows before
-  int* need = start + rows;     // [rows]
-  int* grants = need + rows;    // [kGrants]
+  int* grants = smem;           // [kGrants]
   int* near = grants + kGrants; // [min(pages, kNearRefs)]
+  __shared__ int tails[kPagesMaxRows];  // last page of a row that may have to leave it, else -1
   __shared__ int warp_sums[32];
   __shared__ int s_copies;
   griddep_wait();
   griddep_launch();
+  const int b = threadIdx.x;
   const bool in_near = pages <= kNearRefs;
   const int* counts = in_near ? near : refs;  // as they were before the call
-  if (threadIdx.x == 0) s_copies = 0;
+  if (b == 0) s_copies = 0;
+  int* t = table + (long long)b * cols;
+  int len = 0, want = 0, tail = -1, first = 0, last = 0, fresh = 0;
+  if (b < rows) {
+    len = max(lens[b], 0);
+    want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
+  }
   if (in_near)
-    for (int p = threadIdx.x; p < pages; p += blockDim.x) near[p] = refs[p];
-  for (int b = threadIdx.x; b < rows; b += blockDim.x) {
-    const int len = lens[b];
-    const int want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
-    int t = -1;
-    if (want > 0 && len > 0 && len % block_size != 0 && len / block_size < cols) {
-      t = table[(long long)b * cols + len / block_size];
-      if (t < 0 || t >= pages) t = -1;
+    for (int p = b; p < pages; p += blockDim.x) near[p] = refs[p];
+  if (want > 0) {
+    if (len % block_size != 0 && len / block_size < cols) {
+      tail = t[len / block_size];
+      if (tail < 0 || tail >= pages) tail = -1;
     }
-    tail[b] = t;
+    first = pages_of(len, block_size);
+    last = int(min((long long)cols, ((long long)len + want - 1) / block_size + 1));
+    for (int c = first; c < last; ++c) fresh += t[c] < 0;
   }
+  tails[b] = tail;
   __syncthreads();
-  int carry = 0;
-  for (int b0 = 0; b0 < rows; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    int n = 0;
-    if (b < rows) {
-      const int len = max(lens[b], 0);
-      const int want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
-      const int t = tail[b];
-      if (t >= 0) {
-        // the rows before this one with the same last page will have left it
-        const int held = counts[t];
-        int earlier = 0;
-        if (held > 1)
+  bool leaves = false;
+  if (tail >= 0 && counts[tail] > 1) {
+    // the rows before this one with the same last page will have left it
+    int earlier = 0;
 #pragma unroll 8
-          for (int q = 0; q < b; ++q) earlier += tail[q] == t;
-        n = held - earlier > 1;
-      }
-      if (want > 0) {
-        const long long end = (long long)len + want;
-        const int first = pages_of(len, block_size);
-        const int last = int(min((long long)cols, (end - 1) / block_size + 1));
-        for (int c = first; c < last; ++c) n += table[(long long)b * cols + c] < 0;
-      }
-      need[b] = n;
-    }
-    int total;
-    const int at = block_scan(b < rows ? n : 0, &total, warp_sums);
-    if (b < rows) start[b] = carry + at;
-    carry += total;
+    for (int q = 0; q < b; ++q) earlier += tails[q] == tail;
+    leaves = counts[tail] - earlier > 1;
   }
+  const int need = fresh + leaves;
+  int all, total;
+  const int start = block_scan(need, &all, warp_sums);
   // free pages, lowest first
-  int* list = carry <= kGrants ? grants : free_list;
+  int* list = all <= kGrants ? grants : free_list;
   int found = 0;
-  for (int p0 = 0; p0 < pages && found < carry; p0 += blockDim.x) {
-    const int p = p0 + threadIdx.x;
+  for (int p0 = 0; p0 < pages && found < all; p0 += blockDim.x) {
+    const int p = p0 + b;
     const int is_free = p < pages && counts[p] <= 0;
-    int total;
     const int at = found + block_scan(is_free, &total, warp_sums);
-    if (is_free && at < carry) list[at] = p;
+    if (is_free && at < all) list[at] = p;
     found += total;
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < rows; b += blockDim.x) {
-    const int n = need[b];
-    const bool served = n > 0 && start[b] + n <= found;
-    short_by[b] = served ? 0 : n;
-    if (!served) continue;
-    const int len = max(lens[b], 0);
-    const int want = row_tokens ? row_tokens[b] : tokens;
-    int g = start[b];
-    int* t = table + (long long)b * cols;
-    const int first = pages_of(len, block_size);
-    const int last = int(min((long long)cols, ((long long)len + want - 1) / block_size + 1));
-    int fresh = 0;
-    for (int c = first; c < last; ++c) fresh += t[c] < 0;
-    if (n > fresh) {  // the shared last page comes first
-      const int page = list[g++];
-      int* rec = work + 3 * atomicAdd(&s_copies, 1);
-      rec[0] = tail[b];
-      rec[1] = page;
-      rec[2] = len % block_size;
-      atomicSub(refs + tail[b], 1);
-      refs[page] = 1;
-      t[len / block_size] = page;
-    }
-    for (int c = first; c < last; ++c)
-      if (t[c] < 0) {
+  if (b < rows) {
+    const bool served = start + need <= found;
+    short_by[b] = served ? 0 : need;
+    if (served && need > 0) {
+      int g = start;
+      if (leaves) {  // the shared last page comes first
         const int page = list[g++];
+        int* rec = work + 3 * atomicAdd(&s_copies, 1);
+        rec[0] = tail;
+        rec[1] = page;
+        rec[2] = len % block_size;
+        atomicSub(refs + tail, 1);
         refs[page] = 1;
-        t[c] = page;
+        t[len / block_size] = page;
       }
+      for (int c = first; c < last && fresh > 0; ++c)
+        if (t[c] < 0) {
+          const int page = list[g++];
+          refs[page] = 1;
+          t[c] = page;
+        }
+    }
   }
   __syncthreads();
-  if (threadIdx.x == 0) *copies = s_copies;
+  if (b == 0) *copies = s_copies;
 }
 
 void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, int* refs,
                    int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s) {
   if (rows <= 0) return;
   if (rows > kPagesMaxRows) throw std::runtime_error("pages_reserve: too many rows");
-  auto smem = [](int rows, int pages) { return (int)sizeof(int) * (3 * rows + kGrants + std::min(pages, kNearRefs)); };
-  set_smem_bytes(pages_reserve_kernel, smem(kPagesMaxRows, kNearRefs));
-  launch_k(pages_reserve_kernel, dim3(1), dim3(kIndexThreads), smem(rows, pages <= kNearRefs ? pages : 0), s, table,
-           rows, cols, lens, row_tokens, tokens, refs, pages, block_size, free_list, work, copies, short_by);
+  set_smem_bytes(pages_reserve_kernel, (int)sizeof(int) * (kGrants + kNearRefs));
+  launch_k(pages_reserve_kernel, dim3(1), dim3(kPagesMaxRows),
+           sizeof(int) * (kGrants + (pages <= kNearRefs ? pages : 0)), s, table, rows, cols, lens, row_tokens, tokens,
+           refs, pages, block_size, free_list, work, copies, short_by);
 }
 
 // ------------------------------------------------------------------ free

@@ -336,7 +336,7 @@ void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int
 // Pages of a paged cache shared by several sequences (kv_pages.cu). A plane is [layers][pages][page
 // bytes] with `layer_stride` bytes between layers (base null: no plane). `work` holds (source,
 // destination, tokens) records, `copies` their number.
-constexpr int kPagesMaxRows = 4000;            // rows of one pages_reserve call (shared memory)
+constexpr int kPagesMaxRows = 1024;            // rows of one pages_reserve call (a thread each)
 constexpr int kPagesMaxMarked = 8 * 128 * 1024;  // pages of one pages_pairs call (a bit each in shared memory)
 struct PagePlane {
   void* base = nullptr;

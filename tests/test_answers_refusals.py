@@ -95,7 +95,7 @@ def test_fork_pages(table, lens, parents, refs, bs, says):
     (i32(3, 4), i32(3), i32(3), 1, "more pages than the cache"),
     (i32(3, 4), i32(3), i32(2), -1, "negative"),
     (i32(3, 4), i32(3), i32(2), i32(2), "token count"),
-    (i32(4001, 1), i32(4001), i32(2), 1, "at most 4000 rows"),
+    (i32(1025, 1), i32(1025), i32(2), 1, "at most 1024 rows"),
     (i32(3, 4), i32(3), i32(2), 1, "CUDA"),
 ])
 def test_reserve_pages(table, lens, refs, tokens, says):
@@ -108,7 +108,7 @@ def test_free_and_compact():
     for rows, says in ((i32(2, 2), "rows must be"), (torch.zeros(2), "int32"), (i32(2), "CUDA"), (None, "CUDA")):
         with pytest.raises((ValueError, RuntimeError), match=says):
             ops.free_pages(i32(3, 4), i32(2), rows)
-    assert ops.kernels().LOGPROBS_MAX_TOP == 32 and ops.kernels().PAGES_MAX_ROWS == 4000
+    assert ops.kernels().LOGPROBS_MAX_TOP == 32 and ops.kernels().PAGES_MAX_ROWS == 1024
     for refs, says in ((i32(3), "more pages than the cache"), (i32(2), "CUDA")):
         with pytest.raises((ValueError, RuntimeError), match=says):
             ops.compact_pages(i32(3, 4), refs, CACHE)

@@ -224,18 +224,23 @@ def test_shared_last_page():
             assert torch.equal(data[:, p * 64 + 7:p * 64 + 64], before[:, p * 64 + 7:p * 64 + 64])
 
 
-def test_many_rows_and_pages():
-    """The most rows of one call, more pages than one sweep of the index kernels, no cache rows moved by chance."""
+@pytest.mark.parametrize("pages", [8192, 20000])
+def test_many_rows_and_pages(pages):
+    """The most rows of one call, more pages than one sweep of the index kernels (and than their shared memory)."""
     ops = _ops()
-    rows, pages, bs = ops.kernels().PAGES_MAX_ROWS, 20000, 4
+    rows, bs = ops.kernels().PAGES_MAX_ROWS, 4
     rng = random.Random(5)
     t, n, r = random_state(rng, rows, 3, pages, bs)
     data = torch.randn(1, pages * bs, 2, device=DEV)
     m = Model(t, n, r, [data.cpu()], bs)
     table, lens, refs = ints(t), ints(n), ints(r)
-    short = ops.reserve_pages(table, lens, refs, data, 2, block_size=bs)
-    assert short.cpu().tolist() == m.reserve(2)
-    same(m, table, refs, data, None, "reserve")
+    for tokens in (2, 17):  # the second asks for several pages a row, over four thousand in all
+        if tokens == 17:
+            table = torch.cat([table, torch.full((rows, 5), -1, dtype=torch.int32, device=DEV)], 1).contiguous()
+            m.table = [row + [-1] * 5 for row in m.table]
+        short = ops.reserve_pages(table, lens, refs, data, tokens, block_size=bs)
+        assert short.cpu().tolist() == m.reserve(tokens)
+        same(m, table, refs, data, None, "reserve")
     ops.free_pages(table, refs, ints(list(range(0, rows, 2))))
     m.free(list(range(0, rows, 2)))
     page_map, live = ops.compact_pages(table, refs, data, block_size=bs)
