@@ -12,9 +12,11 @@
 //
 //  * The tensor cores add the products of a K block onto the accumulator and cut the sum off
 //    below its last bit instead of rounding: over long K the logits shrink by about 1e-6 of
-//    their size, all the same way, which shows in the entropy. So K is taken in segments of
-//    1,024, each with an accumulator of its own, and the epilogue adds the segments with
-//    rounding (K = 2,048: entropy off by 1.5e-6 with one accumulator).
+//    their size, all the same way, which shows in the entropy (off by 1.5e-6 of itself at K =
+//    2,048). So K is taken in segments, each with an accumulator of its own, and the epilogue
+//    adds the segments with rounding: segments of 1,024 on CTA pairs (off by 7e-7; one
+//    accumulator would be 2.5% faster under the power limit), of 512 on single CTAs, of 256
+//    where one row tile leaves the epilogue idle anyway (off by 1.5e-7).
 //  * Work items are (128 rows, a range of 64-token units of the vocabulary), rows fastest:
 //    the CTAs that run at the same time read the same range of w, so it comes from memory
 //    once and then from L2, and one row tile's shares are few enough to join cheaply.
@@ -39,7 +41,6 @@ constexpr int kRows = 128;       // rows of a CTA's item
 constexpr int kCols = 256;       // logits of a tile's row
 constexpr int kBox = 64;         // rows of a TMA box of w
 constexpr int kBlockK = 64;
-constexpr int kSegBlocks = 16;   // K blocks of a segment
 constexpr int kXBytes = kRows * kBlockK * 2;
 constexpr int kBoxBytes = kBox * kBlockK * 2;
 constexpr int kHalf = 128;       // columns of an epilogue thread
@@ -71,7 +72,8 @@ SP_DEVI void share_units(const LmParams& p, int share, int& u0, int& u1) {
 
 }  // namespace
 
-template <int CTAS>
+// SEG: K blocks of a segment.
+template <int CTAS, int SEG>
 __global__ void __launch_bounds__(64 + kEpilogue, 1)
     lm_logprobs_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                        const LmParams p) {
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
           const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, min(kTile, u1 - u0) * kUnit);
           for (int kb = 0; kb < blocks; ++kb, ++it) {
             const int buf = tc & 1;
-            if (kb % kSegBlocks == 0) {
+            if (kb % SEG == 0) {
               if (!mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
               tc_fence_after();
             }
@@ -184,11 +186,11 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
             const uint64_t a = sdesc_kmajor_sw128(at), b = sdesc_kmajor_sw128(at + kXBytes);
 #pragma unroll
             for (int k = 0; k < kBlockK / 16; ++k) {
-              const uint32_t more = (kb % kSegBlocks > 0 || k > 0) ? 1u : 0u;
+              const uint32_t more = (kb % SEG > 0 || k > 0) ? 1u : 0u;
               if (CTAS == 2) umma_f16_pair(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
               else umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
             }
-            const bool last = kb % kSegBlocks == kSegBlocks - 1 || kb == blocks - 1;
+            const bool last = kb % SEG == SEG - 1 || kb == blocks - 1;
             if (CTAS == 2) {
               umma_commit_pair(&empty[s]);
               if (last) umma_commit_pair(&tfull[buf]);
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
         // columns of this thread: up to the share's end and the vocabulary's
         const int cols = min(kHalf, min(u1 * kUnit, p.V) - first);
         float v[kHalf];
-        for (int kb = 0; ok && kb < blocks; kb += kSegBlocks, ++tc) {
+        for (int kb = 0; ok && kb < blocks; kb += SEG, ++tc) {
           const int buf = tc & 1;
           ok = __all_sync(0xffffffffu, mbar_wait(&tfull[buf], (tc >> 1) & 1, s_err, p.err, kErrWaitTimeoutEpilogue));
           if (!ok) break;
@@ -376,10 +378,10 @@ LmPlan lm_plan(int T, int V, int num_sms) {
   return l;
 }
 
-template <int CTAS>
+template <int CTAS, int SEG>
 void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, const LmParams& p, int num_sms,
                cudaStream_t s) {
-  auto kern = lm_logprobs_kernel<CTAS>;
+  auto kern = lm_logprobs_kernel<CTAS, SEG>;
   set_smem_bytes(kern, Lm<CTAS>::kSmem);
   prefer_max_smem_carveout(reinterpret_cast<const void*>(kern));
   cudaLaunchConfig_t cfg = {};
@@ -434,8 +436,9 @@ void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int
   CUtensorMap tx, tw;
   make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows, kBlockK);
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
-  if (l.ctas == 2) launch_lm<2>(l, tx, tw, p, num_sms, s);
-  else launch_lm<1>(l, tx, tw, p, num_sms, s);
+  if (l.ctas == 2) launch_lm<2, 16>(l, tx, tw, p, num_sms, s);
+  else if (l.row_tiles > 1) launch_lm<1, 8>(l, tx, tw, p, num_sms, s);
+  else launch_lm<1, 4>(l, tx, tw, p, num_sms, s);
   launch_k(lm_logprobs_join_kernel, dim3((T + 3) / 4), dim3(128), 0, s, (const float4*)workspace, 2 * p.shares,
            p.row_tiles * l.ctas * kRows, T, V, ids, lp, entropy);
 }
