@@ -350,8 +350,15 @@ SP_DEVI void copy_words(const CopyPlane& p, int layer, int src, int dst, int fro
   const long long off = layer * p.layer_stride;
   const int* s = reinterpret_cast<const int*>(p.base + off + (long long)src * p.page_bytes);
   int* d = reinterpret_cast<int*>(p.base + off + (long long)dst * p.page_bytes);
-#pragma unroll 4
-  for (int w = from / 4 + first; w < to / 4; w += step) d[w] = s[w];
+  for (int w = from / 4 + first; w < to / 4; w += 4 * step) {
+    int v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (w + j * step < to / 4) v[j] = s[w + j * step];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (w + j * step < to / 4) d[w + j * step] = v[j];
+  }
 }
 
 // A table's entries through the page map of a compaction.
@@ -406,11 +413,12 @@ __global__ void __launch_bounds__(kCopyThreads)
   char* to[kStages];
   int bytes[kStages];
   bool ok = true;
-  for (int i0 = 0; i0 < n + 1; i0 += kStages) {
+  int issued = 0;
+  for (int i0 = 0; i0 < n + 1 && ok; i0 += kStages) {
 #pragma unroll
     for (int st = 0; st < kStages; ++st) {
       const int i = i0 + st;
-      if (i < n) {
+      if (i < n && ok) {
         // the store that last read this stage: all but the youngest kStages - 2 have been read
         if (i >= kStages) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStages - 2) : "memory");
         const int u = blockIdx.x + i * gridDim.x;
@@ -422,17 +430,19 @@ __global__ void __launch_bounds__(kCopyThreads)
         mbar_arrive_expect_tx(&full[st], bytes[st]);
         if (bytes[st])
           bulk_load(ring + st * kStageBytes, a.base + off + (long long)work[3 * c] * a.page_bytes, bytes[st], &full[st]);
+        issued = i + 1;
       }
       constexpr int kPrev = kStages - 1;
       const int j = i - 1, ps = (st + kPrev) % kStages;
-      if (j >= 0 && j < n) {
-        ok = ok && mbar_wait(&full[ps], (j / kStages) & 1, &s_err, err, kErrWaitTimeoutProducer);
+      if (j >= 0 && j < n && ok) {
+        ok = mbar_wait(&full[ps], (j / kStages) & 1, &s_err, err, kErrWaitTimeoutProducer);
         if (ok && bytes[ps]) bulk_store(to[ps], ring + ps * kStageBytes, bytes[ps]);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
   }
-  for (int j = max(0, n - kStages); j < n && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
+  // after a wait that gave up: loads in flight land before the CTA gives up its memory
+  for (int j = max(0, issued - kStages); j < issued && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 

@@ -329,10 +329,15 @@ constexpr int kLogprobsMaxTop = 32;
 void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,
                     int num_sms, float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s);
 // The same without alternatives from x [T, K] and w [V, K] bf16, logits never in memory
-// (lm_logprobs.cu); the workspace is lm_logprobs_workspace() float4 elements.
-long long lm_logprobs_workspace(int T, int V, int num_sms);
-void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K, const int* ids,
-                 void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s);
+// (lm_logprobs.cu); `workspace` holds lm_plan(...).workspace() float4 elements.
+constexpr int kLmRows = 128;  // rows of a CTA's tile
+struct LmPlan {
+  int ctas = 1, row_tiles = 0, units = 0, shares = 1;
+  long long workspace() const { return 2ll * shares * row_tiles * ctas * kLmRows; }
+};
+LmPlan lm_plan(int T, int V, int num_sms);
+void lm_logprobs(const LmPlan& plan, const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K,
+                 const int* ids, void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s);
 // Pages of a paged cache shared by several sequences (kv_pages.cu). A plane is [layers][pages][page
 // bytes] with `layer_stride` bytes between layers (base null: no plane). `work` holds (source,
 // destination, tokens) records, `copies` their number.

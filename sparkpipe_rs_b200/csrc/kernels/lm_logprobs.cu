@@ -37,7 +37,7 @@ namespace sp {
 
 namespace {
 
-constexpr int kRows = 128;       // rows of a CTA's item
+constexpr int kRows = kLmRows;
 constexpr int kCols = 256;       // logits of a tile's row
 constexpr int kBox = 64;         // rows of a TMA box of w
 constexpr int kBlockK = 64;
@@ -268,10 +268,10 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
           for (int j = 0; j < kHalf; ++j)
             if (j == want && want < cols) given = v[j];
         }
-        float top = v[0];
+        float top[4] = {v[0], v[1], v[2], v[3]};  // four chains of maxima, not one of 128
 #pragma unroll
-        for (int j = 1; j < kHalf; ++j) top = fmaxf(top, v[j]);
-        a.raise(top);
+        for (int j = 4; j < kHalf; ++j) top[j & 3] = fmaxf(top[j & 3], v[j]);
+        a.raise(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
         const float sh = a.shift();
         const u64t shift = pack2(sh, sh);
         u64t s0 = 0, s1 = 0, e0 = 0, e1 = 0;
@@ -348,12 +348,6 @@ __global__ void __launch_bounds__(128) lm_logprobs_join_kernel(const float4* __r
   lp[row] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (given - (empty ? 0.f : m)) - log_s;
 }
 
-namespace {
-
-struct LmPlan {
-  int ctas, row_tiles, units, shares;
-};
-
 // CTA pairs read half as much of w per SM, which lifts 8,192 x 102,400 x 2,048 from 2.83 to
 // 2.46 ms (1,400 TFLOP/s) and 512 rows from 195 to 174 us; below two tiles per SM the single
 // CTAs' finer items win (333 x 10,007 x 1,000: 20 against 24 us). The vocabulary's shares per
@@ -365,7 +359,7 @@ LmPlan lm_plan(int T, int V, int num_sms) {
   l.ctas = T > kRows && tiles >= 2ll * num_sms ? 2 : 1;
   l.row_tiles = (T + kRows * l.ctas - 1) / (kRows * l.ctas);
   l.units = (V + kBox * l.ctas - 1) / (kBox * l.ctas);
-  const int workers = num_sms / l.ctas;
+  const int workers = std::max(1, num_sms / l.ctas);
   long long best = -1;
   for (int s = 1; s <= std::min(l.units, workers); ++s) {
     const long long rounds = ((long long)l.row_tiles * s + workers - 1) / workers;
@@ -379,7 +373,7 @@ LmPlan lm_plan(int T, int V, int num_sms) {
 }
 
 template <int CTAS, int SEG>
-void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, const LmParams& p, int num_sms,
+static void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, const LmParams& p, int num_sms,
                cudaStream_t s) {
   auto kern = lm_logprobs_kernel<CTAS, SEG>;
   set_smem_bytes(kern, Lm<CTAS>::kSmem);
@@ -407,17 +401,9 @@ void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, co
   if (e != cudaSuccess) throw std::runtime_error(std::string("lm_logprobs launch failed: ") + cudaGetErrorString(e));
 }
 
-}  // namespace
-
-long long lm_logprobs_workspace(int T, int V, int num_sms) {
-  const LmPlan l = lm_plan(T, V, num_sms);
-  return 2ll * l.shares * l.row_tiles * l.ctas * kRows;
-}
-
-void lm_logprobs(const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K, const int* ids,
-                 void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s) {
+void lm_logprobs(const LmPlan& l, const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K,
+                 const int* ids, void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s) {
   if (T <= 0) return;
-  const LmPlan l = lm_plan(T, V, num_sms);
   LmParams p = {};
   p.T = T;
   p.V = V;

@@ -41,6 +41,8 @@ class ParallelAnswers:
                  use_graph: bool = True):
         if answers < 1 or max_tokens_per_row < 1:
             raise ValueError("ParallelAnswers: needs an answer and room for its tokens")
+        if max_tokens_per_row > model.cos_sin.shape[0]:
+            raise ValueError(f"ParallelAnswers: the model's positions end at {model.cos_sin.shape[0]}")
         if getattr(model, "ep", None) is not None:
             raise ValueError("ParallelAnswers: one rank only")
         self.model, self.cache, self.n = model, cache, answers

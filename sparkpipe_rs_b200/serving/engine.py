@@ -839,11 +839,12 @@ class LLMEngine:
         if not self.is_cuda or not isinstance(self.model, MLAMoEModel) or self._lockstep is not None:
             raise ValueError("score needs the GPU model on one rank")
         limit = self.ecfg.max_prefill_tokens
+        longest = min(limit, self.ecfg.max_model_len, self.model.cos_sin.shape[0])
         out: list[list[float]] = [[] for _ in prompts]
         todo = []
         for i, p in enumerate(prompts):
-            if len(p) > min(limit, self.ecfg.max_model_len):
-                raise ValueError(f"score: a prompt of {len(p)} tokens exceeds one prefill chunk ({limit}) or the model length")
+            if len(p) > longest:
+                raise ValueError(f"score: a prompt of {len(p)} tokens; one prefill chunk and the model's length allow {longest}")
             if not all(0 <= int(t) < self.cfg.vocab_size for t in p):
                 raise ValueError("score: token ids outside the vocabulary")
             if len(p) > 1:

@@ -164,6 +164,8 @@ def test_answers_refused(model):
     for args in (([], 4), ([1], 0), ([1] * 300, 30), ([4096], 4), ([-1], 4)):
         with pytest.raises(ValueError):
             pa.generate(*args)
+    with pytest.raises(ValueError, match="positions"):
+        type(pa)(model, pa.cache, 2, 1025)
     with pytest.raises(ValueError, match="keep"):
         pa.generate([1, 2], 3, keep=3)
     with pytest.raises(MemoryError, match="prompt"):
