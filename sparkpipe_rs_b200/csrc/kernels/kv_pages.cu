@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   int* grants = smem;           // [kGrants]
   int* near = grants + kGrants; // [min(pages, kNearRefs)]
   __shared__ int tails[kPagesMaxRows];  // last page of a row that may have to leave it, else -1
+  __shared__ bool unserved[kPagesMaxRows];
   __shared__ int warp_sums[32];
   __shared__ int s_copies;
   griddep_wait();
@@ -171,10 +172,17 @@ __global__ void __launch_bounds__(kPagesMaxRows)
     if (is_free && at < all) list[at] = p;
     found += total;
   }
+  const bool served = start + need <= found;
+  unserved[b] = need > 0 && !served;
   __syncthreads();
+  int lacks = served ? 0 : need;
+  if (all > found && need == 0 && tail >= 0 && counts[tail] > 1) {
+    // a row that was to keep the page must not write to it while an earlier one is still there
+    for (int q = 0; q < b; ++q)
+      if (tails[q] == tail && unserved[q]) lacks = 1;
+  }
   if (b < rows) {
-    const bool served = start + need <= found;
-    short_by[b] = served ? 0 : need;
+    short_by[b] = lacks;
     if (served && need > 0) {
       int g = start;
       if (leaves) {  // the shared last page comes first

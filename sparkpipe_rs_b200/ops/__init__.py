@@ -670,9 +670,10 @@ def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, 
     replaced by a private copy of the row's tokens in it (every layer of the cache).
 
     ``tokens``: a number (rows with lens[b] <= 0 are idle and get nothing) or int32 [rows].
-    Rows are served in order, each wholly or not at all; returns int32 [rows], the pages that
-    a row lacks (0: it may be written). The table's width bounds a row. At most
-    PAGES_MAX_ROWS rows."""
+    Rows are served in order, each wholly or not at all; of the rows that share a last page
+    the last one keeps it, once the others have left. Returns int32 [rows], the pages that a
+    row lacks (0: it may be written). The table's width bounds a row; pages that a row has
+    behind its last token are taken to be its own. At most PAGES_MAX_ROWS (1,024) rows."""
     per_row = tokens if isinstance(tokens, torch.Tensor) else None
     short = kernels().reserve_pages(block_table, lens, refs, cache_data, cache_scales, per_row,
                                     0 if per_row is not None else int(tokens), int(block_size))
@@ -689,8 +690,9 @@ def free_pages(block_table, refs, rows=None):
 def compact_pages(block_table, refs, cache_data, block_size=64, cache_scales=None):
     """Moves the live pages (refs > 0) to the front of the cache, in place: with L of them,
     the j-th live page at or behind L moves to the j-th free page before L, in every layer;
-    block_table and refs follow (an entry that names a free page becomes -1). Returns (page_map [pages] int32: each page's new place, -1
-    for a free one, for whatever else holds pages; L as int32 [1])."""
+    block_table and refs follow (an entry that names a free page becomes -1). Returns
+    (page_map [pages] int32: each page's new place, -1 for a free one, for whatever else
+    holds pages; L as int32 [1])."""
     out = kernels().compact_pages(block_table, refs, cache_data, cache_scales, int(block_size))
     _count(2)
     return out

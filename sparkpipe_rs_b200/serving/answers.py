@@ -39,8 +39,8 @@ class ParallelAnswers:
 
     def __init__(self, model: MLAMoEModel, cache: KVCache, answers: int, max_tokens_per_row: int, top_logprobs: int = 0,
                  use_graph: bool = True):
-        if answers < 1 or max_tokens_per_row < 1:
-            raise ValueError("ParallelAnswers: needs an answer and room for its tokens")
+        if not 1 <= answers <= ops.kernels().PAGES_MAX_ROWS or max_tokens_per_row < 1:
+            raise ValueError("ParallelAnswers: 1 to 1,024 answers, and room for their tokens")
         if max_tokens_per_row > model.cos_sin.shape[0]:
             raise ValueError(f"ParallelAnswers: the model's positions end at {model.cos_sin.shape[0]}")
         if getattr(model, "ep", None) is not None:

@@ -57,7 +57,7 @@ class Model:
     def reserve(self, tokens):
         free = [p for p, r in enumerate(self.refs) if r <= 0]
         start_refs = list(self.refs)
-        left, at, short, tails = len(free), 0, [], []
+        left, at, short, tails, stuck = len(free), 0, [], [], []
         for b, row in enumerate(self.table):
             n = max(self.lens[b], 0)
             want = tokens[b] if isinstance(tokens, list) else (tokens if n > 0 else 0)
@@ -71,6 +71,11 @@ class Model:
             need = private + len(fresh)
             ok = at + need <= left
             short.append(0 if ok else need)
+            if need and not ok and col < len(row):
+                stuck.append(row[col] if private else None)
+            # the page that a row was to keep still has an unserved one on it
+            if not need and want > 0 and n % self.bs and col < len(row) and row[col] >= 0 and row[col] in stuck:
+                short[-1] = 1
             if ok and need:
                 g = at
                 if private:
@@ -222,6 +227,19 @@ def test_shared_last_page():
         for p in (0, 1):
             assert torch.equal(data[:, p * 64:p * 64 + 7], before[:, 192:199])
             assert torch.equal(data[:, p * 64 + 7:p * 64 + 64], before[:, p * 64 + 7:p * 64 + 64])
+
+
+def test_no_page_left_for_a_shared_one():
+    """Two rows of different lengths on one page, one page too few: neither may write, and with
+    a free page the first leaves with its tokens and the second keeps the page."""
+    ops = _ops()
+    for pages, short, table in ((1, [1, 1], [[0], [0]]), (2, [0, 0], [[1], [0]])):
+        data, _ = make_cache("bf16", 1, pages, 16, 3)
+        before = data.clone()
+        t, refs = ints([[0], [0]]), ints([2, 0][:pages])
+        assert ops.reserve_pages(t, ints([12, 5]), refs, data, 2, block_size=16).tolist() == short
+        assert t.tolist() == table
+        assert torch.equal(data[:, 16:28], before[:, :12]) if pages == 2 else torch.equal(data, before)
 
 
 @pytest.mark.parametrize("pages", [8192, 20000])
