@@ -51,15 +51,21 @@ template <int CTAS>
 struct Lm {
   static constexpr int kUnit = kBox * CTAS;         // tokens of a unit of the vocabulary
   static constexpr int kTile = kCols / kUnit;       // units of a tile = boxes of w that a CTA loads
-  static constexpr int kStageBytes = kXBytes + kTile * kBoxBytes;
-  static constexpr int kStages = CTAS == 2 ? 6 : 4;
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
 };
+
+// The ring holds as many stages as fit: a stage is the rows of x that there are and the boxes of
+// the largest tile, 48 KB for 128 x 256, 10 KB for a few rows and a share of 64 tokens, where
+// four stages left a K block 0.43 us (the time of a copy) whatever its size.
+constexpr int kMaxStages = 16;
+constexpr int kRing = 224 * 1024;
+constexpr int kSmem = kRing + 1024 + 512;
+static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 
 struct LmParams {
   int T, V, K;
   int row_tiles, units, shares;  // row tiles, units of the vocabulary, shares of a row tile
   int x_bytes;                   // of a box of x: one row tile loads only the rows that there are
+  int stages, stage_bytes;
   const int* ids;
   float4* part;                  // [shares * 2][row_tiles * 128]: m, S, E (log2 units), the given token's logit
   int* err;
@@ -78,19 +84,20 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
     lm_logprobs_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                        const LmParams p) {
   using C = Lm<CTAS>;
-  constexpr int kStages = C::kStages, kStageBytes = C::kStageBytes, kTile = C::kTile, kUnit = C::kUnit;
+  constexpr int kTile = C::kTile, kUnit = C::kUnit;
+  const int stages = p.stages, stage_bytes = p.stage_bytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* tfull = empty + kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kRing);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)cluster_ctarank() : 0;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -126,7 +133,8 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
   if (warp == 0) {
     if (lane == 0) {
       const uint64_t once = policy_evict_first();  // with one row tile, w only passes through L2
-      int it = 0;
+      int s = 0, it = 0;
+      uint32_t phase = 1;
       bool ok = true;
       for (int item = item0; ok && item < items; item += step) {
         int u0, u1;
@@ -135,55 +143,59 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
         for (; ok && u0 < u1; u0 += kTile) {
           const int n = min(kTile, u1 - u0);
           const int col = u0 * kUnit + rank * n * kBox;  // a pair splits the tile's rows of w
-          for (int kb = 0; kb < blocks; ++kb, ++it) {
-            const int s = it % kStages;
-            if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutProducer)) {
+          for (int kb = 0; kb < blocks; ++kb) {
+            if (!mbar_wait(&empty[s], phase, s_err, p.err, kErrWaitTimeoutProducer)) {
               ok = false;
               break;
             }
-            uint8_t* at = smem + s * kStageBytes;
+            uint8_t* at = smem + s * stage_bytes;
             if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (p.x_bytes + n * kBoxBytes));
             if (CTAS == 2) {
               const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
               tma_load_2d_pair(at, &tmX, bar, kb * kBlockK, row);
               for (int i = 0; i < n; ++i)
-                tma_load_2d_pair(at + kXBytes + i * kBoxBytes, &tmW, bar, kb * kBlockK, col + i * kBox);
+                tma_load_2d_pair(at + p.x_bytes + i * kBoxBytes, &tmW, bar, kb * kBlockK, col + i * kBox);
             } else {
               tma_load_2d(at, &tmX, &full[s], kb * kBlockK, row);
               for (int i = 0; i < n; ++i) {
-                uint8_t* box = at + kXBytes + i * kBoxBytes;
+                uint8_t* box = at + p.x_bytes + i * kBoxBytes;
                 if (p.row_tiles == 1) tma_load_2d_hint(box, &tmW, &full[s], kb * kBlockK, col + i * kBox, once);
                 else tma_load_2d(box, &tmW, &full[s], kb * kBlockK, col + i * kBox);
               }
+            }
+            ++it;
+            if (++s == stages) {
+              s = 0;
+              phase ^= 1;
             }
           }
         }
       }
       // loads in flight land before the CTA gives up its memory (a pair's count on its first CTA)
       if (rank == 0)
-        for (int j = max(0, it - kStages); j < it && !ok; ++j) mbar_drain(&full[j % kStages], (j / kStages) & 1);
+        for (int j = max(0, it - stages); j < it && !ok; ++j) mbar_drain(&full[j % stages], (j / stages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      int it = 0, tc = 0;
+      int s = 0, tc = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int item = item0; ok && item < items; item += step) {
         int u0, u1;
         share_units(p, item / p.row_tiles, u0, u1);
         for (; ok && u0 < u1; u0 += kTile) {
           const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, min(kTile, u1 - u0) * kUnit);
-          for (int kb = 0; kb < blocks; ++kb, ++it) {
+          for (int kb = 0; kb < blocks; ++kb) {
             const int buf = tc & 1;
             if (kb % SEG == 0) {
               if (!mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
               tc_fence_after();
             }
-            const int s = it % kStages;
-            if (!mbar_wait(&full[s], (it / kStages) & 1, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
+            if (!mbar_wait(&full[s], phase, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t at = smem_u32(smem + s * kStageBytes);
-            const uint64_t a = sdesc_kmajor_sw128(at), b = sdesc_kmajor_sw128(at + kXBytes);
+            const uint32_t at = smem_u32(smem + s * stage_bytes);
+            const uint64_t a = sdesc_kmajor_sw128(at), b = sdesc_kmajor_sw128(at + p.x_bytes);
 #pragma unroll
             for (int k = 0; k < kBlockK / 16; ++k) {
               const uint32_t more = (kb % SEG > 0 || k > 0) ? 1u : 0u;
@@ -199,6 +211,10 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
               if (last) umma_commit(&tfull[buf]);
             }
             if (last) ++tc;
+            if (++s == stages) {
+              s = 0;
+              phase ^= 1;
+            }
           }
         }
       }
@@ -298,14 +314,16 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
   }
 }
 
-// One warp per row joins its shares; a lane has all its parts under way before it uses one.
-__global__ void __launch_bounds__(128) lm_logprobs_join_kernel(const float4* __restrict__ part, int parts, int pitch,
+// One warp per row joins its shares; a lane has all its parts under way before it uses one. A
+// CTA is one warp: rows' scattered parts are read by as many SMs as there are rows (128 rows x
+// 296 parts: 8.7 us with the kernel before it, 16.7 us with four warps to a CTA).
+__global__ void __launch_bounds__(32) lm_logprobs_join_kernel(const float4* __restrict__ part, int parts, int pitch,
                                                                int T, int V, const int* __restrict__ ids,
                                                                float* __restrict__ lp, float* __restrict__ entropy) {
   constexpr int kAhead = 10;  // 320 parts at once: two for each of 148 CTAs
   griddep_wait();
   griddep_launch();
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = blockIdx.x, lane = threadIdx.x & 31;
   if (row >= T) return;
   const int id = ids[row];
   float m = -INFINITY, given = 0.f;
@@ -376,13 +394,13 @@ template <int CTAS, int SEG>
 static void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, const LmParams& p, int num_sms,
                cudaStream_t s) {
   auto kern = lm_logprobs_kernel<CTAS, SEG>;
-  set_smem_bytes(kern, Lm<CTAS>::kSmem);
+  set_smem_bytes(kern, kSmem);
   prefer_max_smem_carveout(reinterpret_cast<const void*>(kern));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attrs[2];
   cfg.gridDim = dim3(CTAS * (unsigned)std::min<long long>(num_sms / CTAS, (long long)l.row_tiles * l.shares));
   cfg.blockDim = dim3(64 + kEpilogue);
-  cfg.dynamicSmemBytes = Lm<CTAS>::kSmem;
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
   cfg.attrs = attrs;
   if (CTAS == 2) {
@@ -419,13 +437,17 @@ void lm_logprobs(const LmPlan& l, const void* x, long long ldx, const void* w, l
   // MMA's other rows are whatever shared memory held; theirs are results that nobody reads.
   const int x_rows = l.row_tiles * l.ctas == 1 ? (T + 7) / 8 * 8 : kRows;
   p.x_bytes = x_rows * kBlockK * 2;
+  const int boxes = std::min(kCols / (kBox * l.ctas), (l.units + l.shares - 1) / l.shares);
+  p.stage_bytes = p.x_bytes + boxes * kBoxBytes;
+  // the MMA reads 128 rows of x from the last stage too, whatever a box holds
+  p.stages = std::min(kMaxStages, (kRing - std::max(p.stage_bytes, kXBytes)) / p.stage_bytes + 1);
   CUtensorMap tx, tw;
   make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows, kBlockK);
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
   if (l.ctas == 2) launch_lm<2, 16>(l, tx, tw, p, num_sms, s);
   else if (l.row_tiles > 1) launch_lm<1, 8>(l, tx, tw, p, num_sms, s);
   else launch_lm<1, 4>(l, tx, tw, p, num_sms, s);
-  launch_k(lm_logprobs_join_kernel, dim3((T + 3) / 4), dim3(128), 0, s, (const float4*)workspace, 2 * p.shares,
+  launch_k(lm_logprobs_join_kernel, dim3(T), dim3(32), 0, s, (const float4*)workspace, 2 * p.shares,
            p.row_tiles * l.ctas * kRows, T, V, ids, lp, entropy);
 }
 
