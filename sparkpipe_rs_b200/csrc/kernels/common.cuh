@@ -116,6 +116,19 @@ SP_DEVI bool mbar_drain(uint64_t* bar, uint32_t parity) {
   return true;
 }
 
+// One thread of a converged warp, the same one each time. A warp that walks its loop together
+// and issues from this thread keeps addresses and descriptors in uniform registers; in a loop
+// behind `lane == 0` a tcgen05.mma took some 80 clocks to issue, a TMA load 200.
+SP_DEVI bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one));
+  return one != 0;
+}
+
 // ---------------------------------------------------------------- TMA
 SP_DEVI void prefetch_tmap(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory");

@@ -54,8 +54,7 @@ struct Lm {
 };
 
 // The ring holds as many stages as fit: a stage is the rows of x that there are and the boxes of
-// the largest tile, 48 KB for 128 x 256, 10 KB for a few rows and a share of 64 tokens, where
-// four stages left a K block 0.43 us (the time of a copy) whatever its size.
+// the largest tile, 48 KB for 128 x 256, 10 KB for a few rows and a share of 64 tokens.
 constexpr int kMaxStages = 16;
 constexpr int kRing = 224 * 1024;
 constexpr int kSmem = kRing + 1024 + 512;
@@ -131,24 +130,26 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
   const int item0 = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t once = policy_evict_first();  // with one row tile, w only passes through L2
-      int s = 0, it = 0;
-      uint32_t phase = 1;
-      bool ok = true;
-      for (int item = item0; ok && item < items; item += step) {
-        int u0, u1;
-        share_units(p, item / p.row_tiles, u0, u1);
-        const int row = ((item % p.row_tiles) * CTAS + rank) * kRows;
-        for (; ok && u0 < u1; u0 += kTile) {
-          const int n = min(kTile, u1 - u0);
-          const int col = u0 * kUnit + rank * n * kBox;  // a pair splits the tile's rows of w
-          for (int kb = 0; kb < blocks; ++kb) {
-            if (!mbar_wait(&empty[s], phase, s_err, p.err, kErrWaitTimeoutProducer)) {
-              ok = false;
-              break;
-            }
-            uint8_t* at = smem + s * stage_bytes;
+    // The whole warp walks the loop, one thread issues: with `lane == 0` around the loops of both
+    // warps a K block took 0.43 us however little it held, now 0.33 (20.7 us for 700 rows x 3,000
+    // tokens, K = 2,000, was 23.3).
+    const bool one = elect_one();
+    const uint64_t once = policy_evict_first();  // with one row tile, w only passes through L2
+    int s = 0, it = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int item = item0; ok && item < items; item += step) {
+      int u0, u1;
+      share_units(p, item / p.row_tiles, u0, u1);
+      const int row = ((item % p.row_tiles) * CTAS + rank) * kRows;
+      for (; ok && u0 < u1; u0 += kTile) {
+        const int n = min(kTile, u1 - u0);
+        const int col = u0 * kUnit + rank * n * kBox;  // a pair splits the tile's rows of w
+        for (int kb = 0; kb < blocks; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase, s_err, p.err, kErrWaitTimeoutProducer));
+          if (!ok) break;
+          uint8_t* at = smem + s * stage_bytes;
+          if (one) {
             if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (p.x_bytes + n * kBoxBytes));
             if (CTAS == 2) {
               const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
@@ -163,21 +164,23 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
                 else tma_load_2d(box, &tmW, &full[s], kb * kBlockK, col + i * kBox);
               }
             }
-            ++it;
-            if (++s == stages) {
-              s = 0;
-              phase ^= 1;
-            }
+          }
+          ++it;
+          if (++s == stages) {
+            s = 0;
+            phase ^= 1;
           }
         }
       }
-      // loads in flight land before the CTA gives up its memory (a pair's count on its first CTA)
-      if (rank == 0)
-        for (int j = max(0, it - stages); j < it && !ok; ++j) mbar_drain(&full[j % stages], (j / stages) & 1);
     }
+    // loads in flight land before the CTA gives up its memory (a pair's count on its first CTA)
+    if (rank == 0)
+      for (int j = max(0, it - stages); j < it && !ok; ++j) mbar_drain(&full[j % stages], (j / stages) & 1);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool one = elect_one();
+      const uint64_t a0 = sdesc_kmajor_sw128(smem_u32(smem));
       int s = 0, tc = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -188,28 +191,29 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
           const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, min(kTile, u1 - u0) * kUnit);
           for (int kb = 0; kb < blocks; ++kb) {
             const int buf = tc & 1;
-            if (kb % SEG == 0) {
-              if (!mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
-              tc_fence_after();
-            }
-            if (!mbar_wait(&full[s], phase, s_err, p.err, kErrWaitTimeoutMma)) { ok = false; break; }
+            if (kb % SEG == 0)
+              ok = __all_sync(0xffffffffu, mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutMma));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[s], phase, s_err, p.err, kErrWaitTimeoutMma));
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t at = smem_u32(smem + s * stage_bytes);
-            const uint64_t a = sdesc_kmajor_sw128(at), b = sdesc_kmajor_sw128(at + p.x_bytes);
-#pragma unroll
-            for (int k = 0; k < kBlockK / 16; ++k) {
-              const uint32_t more = (kb % SEG > 0 || k > 0) ? 1u : 0u;
-              if (CTAS == 2) umma_f16_pair(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
-              else umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
-            }
+            const uint64_t a = a0 + uint32_t(s * (stage_bytes >> 4)), b = a + (p.x_bytes >> 4);
             const bool last = kb % SEG == SEG - 1 || kb == blocks - 1;
-            if (CTAS == 2) {
-              umma_commit_pair(&empty[s]);
-              if (last) umma_commit_pair(&tfull[buf]);
-            } else {
-              umma_commit(&empty[s]);
-              if (last) umma_commit(&tfull[buf]);
+            if (one) {
+#pragma unroll
+              for (int k = 0; k < kBlockK / 16; ++k) {
+                const uint32_t more = (kb % SEG > 0 || k > 0) ? 1u : 0u;
+                if (CTAS == 2) umma_f16_pair(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
+                else umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
+              }
+              if (CTAS == 2) {
+                umma_commit_pair(&empty[s]);
+                if (last) umma_commit_pair(&tfull[buf]);
+              } else {
+                umma_commit(&empty[s]);
+                if (last) umma_commit(&tfull[buf]);
+              }
             }
+            __syncwarp();
             if (last) ++tc;
             if (++s == stages) {
               s = 0;
