@@ -673,13 +673,15 @@ static void launch(const T* logits, long long ld, int rows, int V, const int* id
 template <typename T>
 static void dispatch(const T* logits, long long ld, int rows, int V, const int* ids, int given, int k, int num_sms,
                      float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
-  // CTAs per row: few rows are split as long as that gives each SM two CTAs at most and each
-  // CTA a whole batch. Split further, a row's join costs more than its stream gains: 64 rows x
-  // 102,400 bf16 with 20 alternatives take 9.7 us in four, 11.1 us in eight; 515 rows 29.9 us
-  // unsplit, 35.1 us in two; one row 7.4 us in four, 6.6 us in eight.
+  // CTAs per row: eight or four as long as that is at most seven CTAs for four SMs (clusters do
+  // not fill the last ones) and each CTA has half a batch. 102,400 bf16 with 20 alternatives:
+  // one row takes 6.6 us in eight, 7.4 in four, 12 unsplit; 32 rows 8.9 in eight, 9.3 in four;
+  // 64 rows 10.5 in four, 12.7 unsplit; 74 rows 13.0 in four, 12.7 unsplit. In two a row's join
+  // eats what its stream gains: 110 rows 13.2 either way, of 32,000 logits 8.2 against 7.1.
   const int batch = kBatch * kThreads * Logits<T>::N;
-  int parts = 1;
-  while (parts < kMaxCluster && (long long)rows * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= batch) parts *= 2;
+  int parts = kMaxCluster;
+  while (parts >= 4 && ((long long)rows * parts * 4 > 7ll * num_sms || V / parts < batch / 2)) parts /= 2;
+  if (parts < 4) parts = 1;
   auto run = [&](auto top, auto cluster) {
     launch<T, decltype(top)::value, decltype(cluster)::value>(logits, ld, rows, V, ids, given, k, parts, lp, entropy,
                                                               top_lp, top_id, s);

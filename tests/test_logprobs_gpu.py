@@ -76,6 +76,17 @@ def test_rows(dtype, T, V, k, pad, shift):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V,pad,shift", [(1, 8191, 0, 0), (2, 8192, 8, 0), (32, 16385, 0, 0), (33, 16391, 3, 1),
+                                           (64, 32767, 2, 5), (65, 32769, 0, 0), (31, 40001, 7, 7)])
+def test_rows_around_the_splits(dtype, T, V, pad, shift):
+    """Rows and lengths at which a row is one, four or eight CTAs' work, the last of them short."""
+    x, ids = make(T, V, dtype, T * 17 + V, pad, shift)
+    ids[0], ids[-1] = V - 1, 0
+    for k in (0, 32):
+        check(_ops().token_logprobs(x, ids, top_k=k), reference(x, ids, k))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [40, 3001, 102400])
 def test_ties_and_order(dtype, V):
     """Equal logits, whole-number logits, rising and falling rows, -0.0 beside 0.0."""
