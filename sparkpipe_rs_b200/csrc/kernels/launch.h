@@ -335,7 +335,7 @@ struct LmPlan {
   int ctas = 1, row_tiles = 0, units = 0, shares = 1;
   long long workspace() const { return 2ll * shares * row_tiles * ctas * kLmRows; }
 };
-LmPlan lm_plan(int T, int V, int num_sms);
+LmPlan lm_plan(int T, int V, int K, int num_sms);
 void lm_logprobs(const LmPlan& plan, const void* x, long long ldx, const void* w, long long ldw, int T, int V, int K,
                  const int* ids, void* workspace, float* lp, float* entropy, int* err, int num_sms, cudaStream_t s);
 // Pages of a paged cache shared by several sequences (kv_pages.cu). A plane is [layers][pages][page

@@ -75,6 +75,14 @@ SP_DEVI void share_units(const LmParams& p, int share, int& u0, int& u1) {
   u1 = int((long long)p.units * (share + 1) / p.shares);
 }
 
+// Units of the next tile: a share's tiles are alike (five units go as 3 + 2: a K block of one unit
+// takes a CTA as long as one of two).
+template <int TILE>
+SP_DEVI int next_tile(int left) {
+  const int tiles = (left + TILE - 1) / TILE;
+  return (left + tiles - 1) / tiles;
+}
+
 }  // namespace
 
 // SEG: K blocks of a segment.
@@ -142,8 +150,8 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
       int u0, u1;
       share_units(p, item / p.row_tiles, u0, u1);
       const int row = ((item % p.row_tiles) * CTAS + rank) * kRows;
-      for (; ok && u0 < u1; u0 += kTile) {
-        const int n = min(kTile, u1 - u0);
+      for (int n; ok && u0 < u1; u0 += n) {
+        n = next_tile<kTile>(u1 - u0);
         const int col = u0 * kUnit + rank * n * kBox;  // a pair splits the tile's rows of w
         for (int kb = 0; kb < blocks; ++kb) {
           ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase, s_err, p.err, kErrWaitTimeoutProducer));
@@ -187,8 +195,9 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
       for (int item = item0; ok && item < items; item += step) {
         int u0, u1;
         share_units(p, item / p.row_tiles, u0, u1);
-        for (; ok && u0 < u1; u0 += kTile) {
-          const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, min(kTile, u1 - u0) * kUnit);
+        for (int n; ok && u0 < u1; u0 += n) {
+          n = next_tile<kTile>(u1 - u0);
+          const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, n * kUnit);
           for (int kb = 0; kb < blocks; ++kb) {
             const int buf = tc & 1;
             if (kb % SEG == 0)
@@ -238,10 +247,11 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
       const int id = row < p.T ? p.ids[row] : -1;
       LogprobSums a;
       float given = 0.f;
-      for (; ok && u0 < u1; u0 += kTile) {
+      for (int n; ok && u0 < u1; u0 += n) {
+        n = next_tile<kTile>(u1 - u0);
         const int first = u0 * kUnit + half * kHalf;
-        // columns of this thread: up to the share's end and the vocabulary's
-        const int cols = min(kHalf, min(u1 * kUnit, p.V) - first);
+        // columns of this thread: up to the tile's end and the vocabulary's
+        const int cols = min(kHalf, min((u0 + n) * kUnit, p.V) - first);
         float v[kHalf];
         for (int kb = 0; ok && kb < blocks; kb += SEG, ++tc) {
           const int buf = tc & 1;
@@ -370,28 +380,62 @@ __global__ void __launch_bounds__(32) lm_logprobs_join_kernel(const float4* __re
   lp[row] = id == -1 ? 0.f : (id < 0 || id >= V || bad) ? NAN : (given - (empty ? 0.f : m)) - log_s;
 }
 
-// CTA pairs read half as much of w per SM, which lifts 8,192 x 102,400 x 2,048 from 2.83 to
-// 2.46 ms (1,400 TFLOP/s) and 512 rows from 195 to 174 us; below two tiles per SM the single
-// CTAs' finer items win (333 x 10,007 x 1,000: 20 against 24 us). The vocabulary's shares per
-// row tile are as many as leave the busiest CTA the fewest units, counting an item's start as
-// one more.
-LmPlan lm_plan(int T, int V, int num_sms) {
+// Clocks that a tile of `n` units keeps a CTA busy: per K block the most of what its warps need
+// to issue (420 a pair, 600 a single CTA), the tensor core's two per column of logits, and its
+// copies at 60 bytes a clock from L2; at least an epilogue's 2,500.
+template <int CTAS>
+static long long tile_clocks(int n, int x_rows, int blocks) {
+  const int copies = (x_rows + n * kBox) * kBlockK * 2 / 60;
+  return std::max<long long>(2500, (long long)blocks * std::max({CTAS == 2 ? 420 : 600, n * Lm<CTAS>::kUnit * 2, copies}));
+}
+
+// The vocabulary's shares per row tile are those that keep the busiest CTA the shortest time, but
+// never shorter than the power limit leaves all of them, which over a longer while is two thirds
+// of the tensor cores' clocks.
+template <int CTAS>
+static LmPlan plan_as(int T, int V, int K, int num_sms, long long& cost) {
+  using C = Lm<CTAS>;
   LmPlan l;
-  const long long tiles = (long long)((T + kRows - 1) / kRows) * ((V + kCols - 1) / kCols);
-  l.ctas = T > kRows && tiles >= 2ll * num_sms ? 2 : 1;
-  l.row_tiles = (T + kRows * l.ctas - 1) / (kRows * l.ctas);
-  l.units = (V + kBox * l.ctas - 1) / (kBox * l.ctas);
-  const int workers = std::max(1, num_sms / l.ctas);
-  long long best = -1;
-  for (int s = 1; s <= std::min(l.units, workers); ++s) {
-    const long long rounds = ((long long)l.row_tiles * s + workers - 1) / workers;
-    const long long cost = rounds * ((l.units + s - 1) / s + 1);
-    if (best < 0 || cost < best) {
-      best = cost;
-      l.shares = s;
+  l.ctas = CTAS;
+  l.row_tiles = (T + kRows * CTAS - 1) / (kRows * CTAS);
+  l.units = (V + C::kUnit - 1) / C::kUnit;
+  const int workers = std::max(1, num_sms / CTAS), blocks = (K + kBlockK - 1) / kBlockK;
+  const long long power = (long long)l.row_tiles * CTAS * l.units * C::kUnit * 2 * blocks / num_sms * 3 / 2;
+  long long clocks[C::kTile + 1];
+  for (int n = 0; n <= C::kTile; ++n) clocks[n] = tile_clocks<CTAS>(n, std::min(T, kRows), blocks);
+  constexpr long long kItemClocks = 5000;
+  cost = -1;
+  for (int rounds = (l.row_tiles + workers - 1) / workers;; ++rounds) {
+    const int most = (int)std::min<long long>({(long long)rounds * workers / l.row_tiles, l.units, workers});
+    const int of_share = (l.units + most - 1) / most, tiles = (of_share + C::kTile - 1) / C::kTile;
+    const int n = of_share / tiles, more = of_share % tiles;  // `more` tiles have n + 1 units
+    const long long busy = kItemClocks + (tiles - more) * clocks[n] + more * clocks[std::min(n + 1, C::kTile)];
+    if (cost < 0 || rounds * busy < cost) {
+      cost = rounds * busy;
+      l.shares = (l.units + of_share - 1) / of_share;
+      // No more shares than keep the busiest as long (10,007 tokens, 61 rows: 13.9 us in 79 shares of
+      // two units, 16.0 in 148), unless a CTA's copies, x again for each tile, are what it waits
+      // for: then all SMs help (102,400 tokens, 61 rows: 73 us in 148 shares, 78.5 in 146; 151,936
+      // tokens, 128 rows: 105 in 148, 109 in 140, but 16 rows 106 in 148, 99 in 140).
+      if (CTAS == 1 && l.row_tiles == 1 && T > 16 && of_share >= C::kTile) l.shares = most;
     }
+    if (most == l.units || most == workers) break;
   }
+  cost = std::max(cost, power);
   return l;
+}
+
+// CTA pairs read half as much of w per SM (8,192 x 102,400 x 2,048 2.07 ms, single CTAs 2.83; 256
+// x 32,000 x 4,096 60 us against 71 to 87, 512 x 10,007 x 1,000 22 against 27), single CTAs' items
+// are finer and the last row tile's empty rows fewer (333 x 10,007 x 1,000 20 us, pairs 22; 300 x
+// 50,000 x 2,048 69 against 75). One row tile stays on single CTAs, whose shorter segments keep
+// the entropy within 2e-7 there.
+LmPlan lm_plan(int T, int V, int K, int num_sms) {
+  long long one = 0, two = 0;
+  const LmPlan single = plan_as<1>(T, V, K, num_sms, one);
+  if (T <= kRows || num_sms < 2) return single;
+  const LmPlan pairs = plan_as<2>(T, V, K, num_sms, two);
+  return two <= one ? pairs : single;
 }
 
 template <int CTAS, int SEG>

@@ -1136,7 +1136,7 @@ std::tuple<Tensor, Tensor> linear_logprobs(const Tensor& x, const Tensor& w, con
   const auto f32 = x.options().dtype(at::kFloat);
   const Tensor lp = at::empty({T}, f32), entropy = at::empty({T}, f32);
   if (T == 0) return {lp, entropy};
-  const sp::LmPlan plan = sp::lm_plan((int)T, (int)V, num_sms());
+  const sp::LmPlan plan = sp::lm_plan((int)T, (int)V, (int)K, num_sms());
   const Tensor work = at::empty({4 * plan.workspace()}, f32);
   sp::lm_logprobs(plan, x.data_ptr(), T > 1 ? x.stride(0) : (K + 7) / 8 * 8, w.data_ptr(), V > 1 ? w.stride(0) : (K + 7) / 8 * 8,
                   (int)T, (int)V, (int)K, ids.data_ptr<int>(), work.data_ptr(), lp.data_ptr<float>(),

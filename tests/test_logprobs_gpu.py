@@ -225,6 +225,14 @@ def test_linear(T, V, K):
     assert ops.status_word() == 0
 
 
+@pytest.mark.parametrize("T,V,K", [(1, 20001, 200), (16, 50001, 72), (17, 50049, 136), (100, 60000, 328), (129, 64, 64),
+                                   (200, 9000, 1104), (257, 130, 3000), (300, 50000, 200), (520, 700, 7168)])
+def test_linear_shares(T, V, K):
+    """Shares of one to seven units in tiles of unequal widths, on single CTAs and pairs; pairs
+    whose second half has no rows or no tokens; segments that end inside K."""
+    test_linear(T, V, K)
+
+
 def test_linear_strides_and_empty():
     ops = _ops()
     g = torch.Generator(device=DEV).manual_seed(3)
