@@ -14,9 +14,11 @@
 //    below its last bit instead of rounding: over long K the logits shrink by about 1e-6 of
 //    their size, all the same way, which shows in the entropy (off by 1.5e-6 of itself at K =
 //    2,048). So K is taken in segments, each with an accumulator of its own, and the epilogue
-//    adds the segments with rounding: segments of 1,024 on CTA pairs (off by 7e-7; one
-//    accumulator would be 2.5% faster under the power limit), of 512 on single CTAs, of 256
-//    where one row tile leaves the epilogue idle anyway (off by 1.5e-7).
+//    adds the segments with rounding: segments of 512 (off by 3e-7 to 6e-7, the more the fewer
+//    tokens there are), of 256 where one row tile leaves the epilogue idle anyway (1.5e-7 to
+//    3e-7), but of 1,024 on CTA pairs over 32,768 tokens and more, where the power limit makes
+//    each pass of the epilogue cost 5% (8,192 x 102,400 x 2,048: 2.47 ms, off by 7e-7; 2.59 ms
+//    in segments of 512; one accumulator would be 2.5% faster still).
 //  * Work items are (128 rows, a range of 64-token units of the vocabulary), rows fastest:
 //    the CTAs that run at the same time read the same range of w, so it comes from memory
 //    once and then from L2, and one row tile's shares are few enough to join cheaply.
@@ -45,6 +47,7 @@ constexpr int kXBytes = kRows * kBlockK * 2;
 constexpr int kBoxBytes = kBox * kBlockK * 2;
 constexpr int kHalf = 128;       // columns of an epilogue thread
 constexpr int kEpilogue = 256;   // epilogue threads
+constexpr int kManyTokens = 32768;  // long segments of K from here on
 
 // CTAs = 2: a pair of CTAs shares a tile of 256 rows x 256 logits, each loads half of w's rows.
 template <int CTAS>
@@ -492,7 +495,8 @@ void lm_logprobs(const LmPlan& l, const void* x, long long ldx, const void* w, l
   CUtensorMap tx, tw;
   make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows, kBlockK);
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
-  if (l.ctas == 2) launch_lm<2, 16>(l, tx, tw, p, num_sms, s);
+  if (l.ctas == 2 && V >= kManyTokens) launch_lm<2, 16>(l, tx, tw, p, num_sms, s);
+  else if (l.ctas == 2) launch_lm<2, 8>(l, tx, tw, p, num_sms, s);
   else if (l.row_tiles > 1) launch_lm<1, 8>(l, tx, tw, p, num_sms, s);
   else launch_lm<1, 4>(l, tx, tw, p, num_sms, s);
   launch_k(lm_logprobs_join_kernel, dim3(T), dim3(32), 0, s, (const float4*)workspace, 2 * p.shares,
