@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -67,6 +68,7 @@ struct LmParams {
   int T, V, K;
   int row_tiles, units, shares;  // row tiles, units of the vocabulary, shares of a row tile
   int x_bytes;                   // of a box of x: one row tile loads only the rows that there are
+  int block_bytes;               // of a K block in the ring: x and the boxes of w
   int stages, stage_bytes;
   const int* ids;
   float4* part;                  // [shares * 2][row_tiles * 128]: m, S, E (log2 units), the given token's logit
@@ -88,8 +90,8 @@ SP_DEVI int next_tile(int left) {
 
 }  // namespace
 
-// SEG: K blocks of a segment.
-template <int CTAS, int SEG>
+// SEG: K blocks of a segment, PER: of a stage of the ring.
+template <int CTAS, int SEG, int PER>
 __global__ void __launch_bounds__(64 + kEpilogue, 1)
     lm_logprobs_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                        const LmParams p) {
@@ -142,8 +144,8 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
 
   if (warp == 0) {
     // The whole warp walks the loop, one thread issues: with `lane == 0` around the loops of both
-    // warps a K block took 0.43 us however little it held, now 0.33 (20.7 us for 700 rows x 3,000
-    // tokens, K = 2,000, was 23.3).
+    // warps a K block took 0.43 us however little it held, so 0.33 (700 rows x 3,000 tokens, K =
+    // 2,000: 23.3 and 20.7 us).
     const bool one = elect_one();
     const uint64_t once = policy_evict_first();  // with one row tile, w only passes through L2
     int s = 0, it = 0;
@@ -156,23 +158,28 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
       for (int n; ok && u0 < u1; u0 += n) {
         n = next_tile<kTile>(u1 - u0);
         const int col = u0 * kUnit + rank * n * kBox;  // a pair splits the tile's rows of w
-        for (int kb = 0; kb < blocks; ++kb) {
+        for (int kb = 0; kb < blocks; kb += PER) {
           ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase, s_err, p.err, kErrWaitTimeoutProducer));
           if (!ok) break;
-          uint8_t* at = smem + s * stage_bytes;
           if (one) {
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (p.x_bytes + n * kBoxBytes));
-            if (CTAS == 2) {
-              const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-              tma_load_2d_pair(at, &tmX, bar, kb * kBlockK, row);
-              for (int i = 0; i < n; ++i)
-                tma_load_2d_pair(at + p.x_bytes + i * kBoxBytes, &tmW, bar, kb * kBlockK, col + i * kBox);
-            } else {
-              tma_load_2d(at, &tmX, &full[s], kb * kBlockK, row);
-              for (int i = 0; i < n; ++i) {
-                uint8_t* box = at + p.x_bytes + i * kBoxBytes;
-                if (p.row_tiles == 1) tma_load_2d_hint(box, &tmW, &full[s], kb * kBlockK, col + i * kBox, once);
-                else tma_load_2d(box, &tmW, &full[s], kb * kBlockK, col + i * kBox);
+            const int end = PER == 1 ? kb + 1 : min(kb + PER, blocks);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], (end - kb) * CTAS * (p.x_bytes + n * kBoxBytes));
+            uint8_t* at = smem + s * stage_bytes;
+            const uint32_t bar = CTAS == 2 ? mapa_shared(smem_u32(&full[s]), 0) : 0;
+#pragma unroll
+            for (int b = kb; b < kb + PER; ++b, at += p.block_bytes) {
+              if (PER > 1 && b >= end) break;
+              if (CTAS == 2) {
+                tma_load_2d_pair(at, &tmX, bar, b * kBlockK, row);
+                for (int i = 0; i < n; ++i)
+                  tma_load_2d_pair(at + p.x_bytes + i * kBoxBytes, &tmW, bar, b * kBlockK, col + i * kBox);
+              } else {
+                tma_load_2d(at, &tmX, &full[s], b * kBlockK, row);
+                for (int i = 0; i < n; ++i) {
+                  uint8_t* box = at + p.x_bytes + i * kBoxBytes;
+                  if (p.row_tiles == 1) tma_load_2d_hint(box, &tmW, &full[s], b * kBlockK, col + i * kBox, once);
+                  else tma_load_2d(box, &tmW, &full[s], b * kBlockK, col + i * kBox);
+                }
               }
             }
           }
@@ -201,7 +208,7 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
         for (int n; ok && u0 < u1; u0 += n) {
           n = next_tile<kTile>(u1 - u0);
           const uint32_t idesc = idesc_bf16_f32(CTAS * kRows, n * kUnit);
-          for (int kb = 0; kb < blocks; ++kb) {
+          for (int kb = 0; kb < blocks; kb += PER) {
             const int buf = tc & 1;
             if (kb % SEG == 0)
               ok = __all_sync(0xffffffffu, mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1, s_err, p.err, kErrWaitTimeoutMma));
@@ -209,13 +216,18 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
             if (!ok) break;
             tc_fence_after();
             const uint64_t a = a0 + uint32_t(s * (stage_bytes >> 4)), b = a + (p.x_bytes >> 4);
-            const bool last = kb % SEG == SEG - 1 || kb == blocks - 1;
+            const uint32_t block = p.block_bytes >> 4;
+            const bool last = (kb + PER) % SEG == 0 || kb + PER >= blocks;
             if (one) {
 #pragma unroll
-              for (int k = 0; k < kBlockK / 16; ++k) {
-                const uint32_t more = (kb % SEG > 0 || k > 0) ? 1u : 0u;
-                if (CTAS == 2) umma_f16_pair(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
-                else umma_f16(tmem + buf * kCols, a + 2 * k, b + 2 * k, idesc, more);
+              for (int j = 0; j < PER; ++j) {
+                if (j > 0 && kb + j >= blocks) break;
+#pragma unroll
+                for (int k = 0; k < kBlockK / 16; ++k) {
+                  const uint32_t more = (kb % SEG > 0 || j + k > 0) ? 1u : 0u;
+                  if (CTAS == 2) umma_f16_pair(tmem + buf * kCols, a + j * block + 2 * k, b + j * block + 2 * k, idesc, more);
+                  else umma_f16(tmem + buf * kCols, a + j * block + 2 * k, b + j * block + 2 * k, idesc, more);
+                }
               }
               if (CTAS == 2) {
                 umma_commit_pair(&empty[s]);
@@ -384,7 +396,7 @@ __global__ void __launch_bounds__(32) lm_logprobs_join_kernel(const float4* __re
 }
 
 // Clocks that a tile of `n` units keeps a CTA busy: per K block the most of what its warps need
-// to issue (420 a pair, 600 a single CTA), the tensor core's two per column of logits, and its
+// to issue (420 a pair, 600 a single CTA; less in stages of two blocks), the tensor core's two per column of logits, and its
 // copies at 60 bytes a clock from L2; at least an epilogue's 2,500.
 template <int CTAS>
 static long long tile_clocks(int n, int x_rows, int blocks) {
@@ -441,10 +453,10 @@ LmPlan lm_plan(int T, int V, int K, int num_sms) {
   return two <= one ? pairs : single;
 }
 
-template <int CTAS, int SEG>
+template <int CTAS, int SEG, int PER>
 static void launch_lm(const LmPlan& l, const CUtensorMap& tx, const CUtensorMap& tw, const LmParams& p, int num_sms,
                cudaStream_t s) {
-  auto kern = lm_logprobs_kernel<CTAS, SEG>;
+  auto kern = lm_logprobs_kernel<CTAS, SEG, PER>;
   set_smem_bytes(kern, kSmem);
   prefer_max_smem_carveout(reinterpret_cast<const void*>(kern));
   cudaLaunchConfig_t cfg = {};
@@ -489,16 +501,27 @@ void lm_logprobs(const LmPlan& l, const void* x, long long ldx, const void* w, l
   const int x_rows = l.row_tiles * l.ctas == 1 ? (T + 7) / 8 * 8 : kRows;
   p.x_bytes = x_rows * kBlockK * 2;
   const int boxes = std::min(kCols / (kBox * l.ctas), (l.units + l.shares - 1) / l.shares);
-  p.stage_bytes = p.x_bytes + boxes * kBoxBytes;
-  // the MMA reads 128 rows of x from the last stage too, whatever a box holds
-  p.stages = std::min(kMaxStages, (kRing - std::max(p.stage_bytes, kXBytes)) / p.stage_bytes + 1);
+  p.block_bytes = p.x_bytes + boxes * kBoxBytes;
+  const bool many = l.ctas == 2 && V >= kManyTokens;
+  // Stages of two K blocks where four fit: a narrow share's K block costs what its warps need to
+  // issue it, half of which is the stage's (9,472 tokens, 16 rows: 0.33 us a block, in twos 0.26).
+  const int per = !many && 8 * p.block_bytes <= kRing ? 2 : 1;
+  p.stage_bytes = per * p.block_bytes;
+  // the MMA reads 128 rows of x from the last block too, whatever a box holds
+  const int behind = (per - 1) * p.block_bytes + std::max(p.block_bytes, kXBytes);
+  p.stages = std::min(kMaxStages, (kRing - behind) / p.stage_bytes + 1);
   CUtensorMap tx, tw;
   make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows, kBlockK);
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
-  if (l.ctas == 2 && V >= kManyTokens) launch_lm<2, 16>(l, tx, tw, p, num_sms, s);
-  else if (l.ctas == 2) launch_lm<2, 8>(l, tx, tw, p, num_sms, s);
-  else if (l.row_tiles > 1) launch_lm<1, 8>(l, tx, tw, p, num_sms, s);
-  else launch_lm<1, 4>(l, tx, tw, p, num_sms, s);
+  auto run = [&](auto two) {
+    constexpr int PER = decltype(two)::value ? 2 : 1;
+    if (l.ctas == 2) launch_lm<2, 8, PER>(l, tx, tw, p, num_sms, s);
+    else if (l.row_tiles > 1) launch_lm<1, 8, PER>(l, tx, tw, p, num_sms, s);
+    else launch_lm<1, 4, PER>(l, tx, tw, p, num_sms, s);
+  };
+  if (many) launch_lm<2, 16, 1>(l, tx, tw, p, num_sms, s);
+  else if (per == 2) run(std::true_type{});
+  else run(std::false_type{});
   launch_k(lm_logprobs_join_kernel, dim3(T), dim3(32), 0, s, (const float4*)workspace, 2 * p.shares,
            p.row_tiles * l.ctas * kRows, T, V, ids, lp, entropy);
 }
