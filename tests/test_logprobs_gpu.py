@@ -87,6 +87,20 @@ def test_rows_around_the_splits(dtype, T, V, pad, shift):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,shift", [(32, 0), (63, 1), (200, 0), (256, 3), (517, 0), (556, 5), (1000, 0), (1091, 2),
+                                     (2048, 0), (2111, 63)])
+def test_short_rows(dtype, V, shift):
+    """Rows of few vectors, where groups of threads are small: whole, masked to a few logits, and with ties."""
+    x, ids = make(48, V, dtype, V + shift, 0, shift)
+    x = x.clone() if shift == 0 else x
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x[16:32].masked_fill_(torch.rand(16, V, device=DEV, generator=g) < 0.9, -INF)
+    x[32:].copy_(torch.randint(-3, 4, (16, V), device=DEV, generator=g).to(dtype))
+    for k in (1, 20, 32):
+        check(_ops().token_logprobs(x, ids, top_k=k), reference(x, ids, k))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [40, 3001, 102400])
 def test_ties_and_order(dtype, V):
     """Equal logits, whole-number logits, rising and falling rows, -0.0 beside 0.0."""
