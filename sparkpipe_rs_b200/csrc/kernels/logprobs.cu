@@ -42,16 +42,14 @@ namespace sp {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kLong = 256, kShort = 64;  // threads of a row's CTA
 // 64 registers, which hold a batch and the next one's loads (8,192 rows x 102,400 with 20
 // alternatives: 323 us, 346 us without the loads ahead; with 80 registers 342 us, with 48 and
 // half as large batches 336 us)
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 4;     // of 256 threads
 constexpr int kBatch = 4;         // 16-byte vectors of a batch, in flight together
 constexpr int kSlots = 16;        // recorded batch maxima of a thread (several batches each in longer rows)
 constexpr int kGroups = 64;
-constexpr int kGroupThreads = kThreads / kGroups;
 constexpr int kList = 1024;       // logits at or above the floor
 constexpr int kHot = 512;         // (thread, slot) entries whose batches reach it
 constexpr int kMaxCluster = 8;
@@ -203,7 +201,7 @@ SP_DEVI bool before(float v, int i, float w, int j) { return v > w || (v == w &&
 // whole vector (at most one each per thread), vectors in between. Vectors that start with a
 // line let a warp's load touch four lines, not five: 515 rows x 129,281 fp32 went from 64 to
 // 57 us (129,280, whose rows all start with a line: 52 us).
-template <typename T>
+template <typename T, int THREADS>
 struct Part {
   const T* row;
   const uint4* body;
@@ -236,10 +234,10 @@ struct Part {
     for (int b = b0; b < b1; ++b) {
       uint4 v[kBatch];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) v[i] = vector(v0 + (b * kBatch + i) * kThreads + threadIdx.x);
+      for (int i = 0; i < kBatch; ++i) v[i] = vector(v0 + (b * kBatch + i) * THREADS + threadIdx.x);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int at = first + (v0 + (b * kBatch + i) * kThreads + (int)threadIdx.x) * Logits<T>::N;
+        const int at = first + (v0 + (b * kBatch + i) * THREADS + (int)threadIdx.x) * Logits<T>::N;
 #pragma unroll
         for (int j = 0; j < Logits<T>::N / 2; ++j) {
           float x, y;
@@ -262,10 +260,11 @@ struct Stat {
   double s, e;
 };
 
+template <int THREADS>
 struct Shared {
-  float slot[kSlots][kThreads];
+  float slot[kSlots][THREADS];
   float group[kGroups];            // maxima of four threads' logits each (of the whole cluster)
-  Stat stat[kMaxCluster * kWarps]; // the cluster's warps (first CTA)
+  Stat stat[kMaxCluster * (THREADS / 32)]; // the cluster's warps (first CTA)
   float floor;
   float base, log_s;               // the row's maximum (0 for an empty row) and ln S
   int bad;
@@ -296,7 +295,8 @@ SP_DEVI int add_s32(int* p, int v, int q) {
 }
 
 // Joins the warps' sums; every lane of the calling warp gets the row's (m, S, E).
-SP_DEVI void join_stats(const Shared& sh, int n, float& m, double& s, double& e) {
+template <int THREADS>
+SP_DEVI void join_stats(const Shared<THREADS>& sh, int n, float& m, double& s, double& e) {
   const int lane = threadIdx.x & 31;
   m = -INFINITY;
   for (int i = lane; i < n; i += 32) m = fmaxf(m, sh.stat[i].m);
@@ -319,8 +319,9 @@ SP_DEVI void join_stats(const Shared& sh, int n, float& m, double& s, double& e)
 // More logits reach the floor than the list holds: each thread offers its best one not
 // yet taken, the CTA takes the best of these, k times. The next offer of the thread whose
 // one was taken is found by its whole warp.
-template <typename T>
-__device__ __noinline__ void pick_rounds(const Part<T>& part, int nb, int k, Shared& sh) {
+template <typename T, int THREADS>
+__device__ __noinline__ void pick_rounds(const Part<T, THREADS>& part, int nb, int k, Shared<THREADS>& sh) {
+  constexpr int WARPS = THREADS / 32;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   float best = -INFINITY;
   int at = kNone;
@@ -347,12 +348,12 @@ __device__ __noinline__ void pick_rounds(const Part<T>& part, int nb, int k, Sha
       sh.id[w] = pi;
     }
     __syncthreads();
-    for (int i = 0; i < kWarps; ++i)
+    for (int i = 0; i < WARPS; ++i)
       if (before(sh.v[i], sh.id[i], pv, pi)) { pv = sh.v[i]; pi = sh.id[i]; }
     if (pi == kNone) break;  // the same for every thread
     if (threadIdx.x == 0) {
-      sh.v[kWarps + r] = pv;
-      sh.id[kWarps + r] = pi;
+      sh.v[WARPS + r] = pv;
+      sh.id[WARPS + r] = pi;
       sh.n = r + 1;
     }
     const unsigned taken = __ballot_sync(0xffffffffu, at == pi);
@@ -363,7 +364,7 @@ __device__ __noinline__ void pick_rounds(const Part<T>& part, int nb, int k, Sha
       auto next = [&](float v, int i) {
         if (v != -INFINITY && i >= 0 && before(pv, pi, v, i) && before(v, i, nv, ni)) { nv = v; ni = i; }
       };
-      for (int v = part.v0 + w * 32 + from + lane * kThreads; v < part.v1; v += 32 * kThreads) {
+      for (int v = part.v0 + w * 32 + from + lane * THREADS; v < part.v1; v += 32 * THREADS) {
         const uint4 q = __ldg(part.body + v);
 #pragma unroll
         for (int j = 0; j < Logits<T>::N / 2; ++j) {
@@ -387,13 +388,14 @@ __device__ __noinline__ void pick_rounds(const Part<T>& part, int nb, int k, Sha
 }  // namespace
 
 // One row per cluster of `parts` CTAs (1: no cluster).
-template <typename T, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+template <typename T, bool TOP, bool CLUSTER, int THREADS>
+__global__ void __launch_bounds__(THREADS, kCtasPerSm * kLong / THREADS)
     token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const int* __restrict__ ids, int given,
                           int k, int parts, float* __restrict__ lp, float* __restrict__ entropy,
                           float* __restrict__ top_lp, int* __restrict__ top_id) {
   extern __shared__ __align__(16) uint8_t smem[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  constexpr int WARPS = THREADS / 32, GROUP = THREADS / kGroups;
+  Shared<THREADS>& sh = *reinterpret_cast<Shared<THREADS>*>(smem);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int rank = CLUSTER ? (int)cluster_ctarank() : 0;
   const long long row = CLUSTER ? blockIdx.x / parts : blockIdx.x;
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   griddep_wait();
   griddep_launch();
   const T* x = logits + row * ld;
-  const Part<T> part(x, V, rank, CLUSTER ? parts : 1);
+  const Part<T, THREADS> part(x, V, rank, CLUSTER ? parts : 1);
   // the first given tokens' logits, on their way while the row streams
   int id = -1;
   float xid = 0.f;
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     id = ids[row * given + threadIdx.x];
     if (id >= 0 && id < V) xid = Logits<T>::value(x[id]);
   }
-  const int nb = (part.v1 - part.v0 + kBatch * kThreads - 1) / (kBatch * kThreads);
+  const int nb = (part.v1 - part.v0 + kBatch * THREADS - 1) / (kBatch * THREADS);
   const int per_slot = (nb + kSlots - 1) / kSlots;
 
   LogprobSums a;
@@ -443,24 +445,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
     }
   };
-  const int whole = (part.v1 - part.v0) / (kBatch * kThreads);
+  const int whole = (part.v1 - part.v0) / (kBatch * THREADS);
   const uint4* src = part.body + part.v0 + threadIdx.x;
   // the next batch's loads go out before this one's arithmetic
   uint4 nx[kBatch];
 #pragma unroll
-  for (int i = 0; i < kBatch; ++i) nx[i] = part.vector(part.v0 + i * kThreads + threadIdx.x);
+  for (int i = 0; i < kBatch; ++i) nx[i] = part.vector(part.v0 + i * THREADS + threadIdx.x);
 #pragma unroll 1
   for (int b = 0; b < whole; ++b) {
     uint4 v[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) v[i] = nx[i];
-    src += kBatch * kThreads;
+    src += kBatch * THREADS;
     if (b + 1 < whole) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) nx[i] = __ldg(src + i * kThreads);
+      for (int i = 0; i < kBatch; ++i) nx[i] = __ldg(src + i * THREADS);
     } else {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) nx[i] = part.vector(part.v0 + (whole * kBatch + i) * kThreads + threadIdx.x);
+      for (int i = 0; i < kBatch; ++i) nx[i] = part.vector(part.v0 + (whole * kBatch + i) * THREADS + threadIdx.x);
     }
     take(v);
   }
@@ -486,15 +488,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     // Short rows have a vector for few threads: groups of one or two, that k of them have a
     // logit (2,001 rows x 556 with 20 alternatives: 21 us, in fours 229).
     const int vectors = part.v1 - part.v0;
-    const int wide = vectors <= kGroups ? 1 : vectors <= 2 * kGroups ? 2 : kGroupThreads;
+    const int wide = min(GROUP, vectors <= kGroups ? 1 : vectors <= 2 * kGroups ? 2 : GROUP);
     for (int o = 1; o < wide; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane % wide == 0 && threadIdx.x / wide < kGroups) sh.group[threadIdx.x / wide] = m;
   }
   if (TOP && CLUSTER) {
-    const int wide = kGroupThreads * parts;  // threads of a group, at most a warp
+    const int wide = GROUP * parts;  // threads of a group, at most a warp
     for (int o = 1; o < wide; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane % wide == 0)
-      for (int q = 0; q < parts; ++q) st_f32(&sh.group[(rank * kThreads + threadIdx.x) / wide], m, q);
+      for (int q = 0; q < parts; ++q) st_f32(&sh.group[(rank * THREADS + threadIdx.x) / wide], m, q);
   }
   m = warp_max(m);
   {
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       e += __shfl_xor_sync(0xffffffffu, e, o);
     }
     if (lane == 0) {
-      Stat* t = &sh.stat[rank * kWarps + w];
+      Stat* t = &sh.stat[rank * WARPS + w];
       st_f32(&t->m, m, first);
       st_f64(&t->s, s, first);
       st_f64(&t->e, e, first);
@@ -518,9 +520,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   else __syncthreads();
 
   // the join by the last warp of the first CTA, the floor by the first warp of each
-  if (rank == 0 && w == kWarps - 1) {
+  if (rank == 0 && w == WARPS - 1) {
     double s, e;
-    join_stats(sh, (CLUSTER ? parts : 1) * kWarps, m, s, e);
+    join_stats(sh, (CLUSTER ? parts : 1) * WARPS, m, s, e);
     if (lane == 0) {
       const bool bad = s != s, empty = !bad && s == 0.0;
       const float log_s = empty ? 0.f : s < 2.0 ? log1pf(float(s - 1.0)) : logf(float(s));
@@ -561,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int q = 0; q < slot; ++q)
         if (sh.slot[q][threadIdx.x] >= floor) {
           const int at = atomicAdd(&sh.hot_n, 1);
-          if (at < kHot) sh.hot[at] = q * kThreads + threadIdx.x;
+          if (at < kHot) sh.hot[at] = q * THREADS + threadIdx.x;
         }
       if (fmaxf(one, two) >= floor) part.singles(see);
     }
@@ -573,20 +575,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     } else {
       constexpr int N = Logits<T>::N, kAhead = 4;
       const int pieces = (per_slot * kBatch * N + 31) / 32;  // of an entry, a logit per lane
-      for (int i0 = w; i0 < entries * pieces; i0 += kAhead * kWarps) {
+      for (int i0 = w; i0 < entries * pieces; i0 += kAhead * WARPS) {
         float v[kAhead];
         int at[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {  // loads first: they come from L2 or memory
-          const int i = i0 + u * kWarps;
+          const int i = i0 + u * WARPS;
           at[u] = -1;
           v[u] = -INFINITY;
           if (i < entries * pieces) {
             const int entry = pieces == 1 ? i : i / pieces;
-            const int t = sh.hot[entry] % kThreads, q = sh.hot[entry] / kThreads;
+            const int t = sh.hot[entry] % THREADS, q = sh.hot[entry] / THREADS;
             const int j = (i - entry * pieces) * 32 + lane;
             const int b = q * per_slot * kBatch + j / N;  // the thread's vector
-            const int vec = part.v0 + b * kThreads + t;
+            const int vec = part.v0 + b * THREADS + t;
             if (j < per_slot * kBatch * N && b < nb * kBatch && vec < part.v1) {
               at[u] = part.first + vec * N + j % N;
               v[u] = Logits<T>::value(x[at[u]]);
@@ -608,8 +610,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 
   const bool bad = sh.bad;
   const float base = sh.base, log_s = sh.log_s;
-  for (int j = threadIdx.x; j < given; j += kThreads) {
-    if (j >= kThreads) {
+  for (int j = threadIdx.x; j < given; j += THREADS) {
+    if (j >= THREADS) {
       id = ids[row * given + j];
       if (id >= 0 && id < V) xid = Logits<T>::value(x[id]);
     }
@@ -619,14 +621,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     int base_at = 0;
     if (n > kList) {
       __syncthreads();  // every warp has read sh.n
-      const Part<T> whole(x, V, 0, 1);
+      const Part<T, THREADS> whole(x, V, 0, 1);
       if (threadIdx.x == 0) sh.n = 0;
-      pick_rounds(whole, (whole.v1 - whole.v0 + kBatch * kThreads - 1) / (kBatch * kThreads), k, sh);
+      pick_rounds(whole, (whole.v1 - whole.v0 + kBatch * THREADS - 1) / (kBatch * THREADS), k, sh);
       n = sh.n;
-      base_at = kWarps;
+      base_at = WARPS;
     }
     // a logit's place is how many rank before it
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
       const float v = sh.v[base_at + i];
       const int at = sh.id[base_at + i];
       int r = 0;
@@ -637,23 +639,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         top_lp[row * k + r] = bad ? NAN : (v - base) - log_s;
       }
     }
-    for (int r = n + threadIdx.x; r < k; r += kThreads) {
+    for (int r = n + threadIdx.x; r < k; r += THREADS) {
       top_id[row * k + r] = -1;
       top_lp[row * k + r] = bad ? NAN : -INFINITY;
     }
   }
 }
 
-template <typename T, bool TOP, bool CLUSTER>
+template <typename T, bool TOP, bool CLUSTER, int THREADS>
 static void launch(const T* logits, long long ld, int rows, int V, const int* ids, int given, int k, int parts,
                    float* lp, float* entropy, float* top_lp, int* top_id, cudaStream_t s) {
-  auto kern = token_logprobs_kernel<T, TOP, CLUSTER>;
+  auto kern = token_logprobs_kernel<T, TOP, CLUSTER, THREADS>;
   prefer_max_smem_carveout(reinterpret_cast<const void*>(kern));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attrs[2];
   cfg.gridDim = dim3((unsigned)(rows * parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = sizeof(Shared<THREADS>);
   cfg.stream = s;
   cfg.attrs = attrs;
   if (CLUSTER) {
@@ -681,18 +683,27 @@ static void dispatch(const T* logits, long long ld, int rows, int V, const int* 
   // one row takes 6.6 us in eight, 7.4 in four, 12 unsplit; 32 rows 8.9 in eight, 9.3 in four;
   // 64 rows 10.5 in four, 12.7 unsplit; 74 rows 13.0 in four, 12.7 unsplit. In two a row's join
   // eats what its stream gains: 110 rows 13.2 either way, of 32,000 logits 8.2 against 7.1.
-  const int batch = kBatch * kThreads * Logits<T>::N;
+  const int batch = kBatch * kLong * Logits<T>::N;
   int parts = kMaxCluster;
   while (parts >= 4 && ((long long)rows * parts * 4 > 7ll * num_sms || V / parts < batch / 2)) parts /= 2;
   if (parts < 4) parts = 1;
-  auto run = [&](auto top, auto cluster) {
-    launch<T, decltype(top)::value, decltype(cluster)::value>(logits, ld, rows, V, ids, given, k, parts, lp, entropy,
-                                                              top_lp, top_id, s);
+  // More short rows than the SMs hold at once take 64 threads each, which leave and are followed
+  // sooner (bf16, 20 alternatives): 8,192 rows x 1,000 43 us, in 256 threads 74; 8,192 x 16,384 86
+  // and 112; 2,001 x 16,384 26 and 29, but 1,200 x 16,384 23 and 20, 600 x 8,192 12.7 and 11.5,
+  // 8,192 x 65,536 266 and 220.
+  const int vectors = V / Logits<T>::N;
+  const bool small = parts == 1 && ((rows > kCtasPerSm * num_sms && vectors <= 512) ||
+                                    (rows > 3 * kCtasPerSm * num_sms && vectors <= 2048));
+  auto run = [&](auto top, auto cluster, auto threads) {
+    launch<T, decltype(top)::value, decltype(cluster)::value, decltype(threads)::value>(
+        logits, ld, rows, V, ids, given, k, parts, lp, entropy, top_lp, top_id, s);
   };
   using Yes = std::true_type;
   using No = std::false_type;
-  if (k > 0) parts > 1 ? run(Yes{}, Yes{}) : run(Yes{}, No{});
-  else parts > 1 ? run(No{}, Yes{}) : run(No{}, No{});
+  const std::integral_constant<int, kLong> wide;
+  const std::integral_constant<int, kShort> narrow;
+  if (k > 0) parts > 1 ? run(Yes{}, Yes{}, wide) : small ? run(Yes{}, No{}, narrow) : run(Yes{}, No{}, wide);
+  else parts > 1 ? run(No{}, Yes{}, wide) : small ? run(No{}, No{}, narrow) : run(No{}, No{}, wide);
 }
 
 void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V, const int* ids, int given, int k,

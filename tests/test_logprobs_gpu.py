@@ -101,6 +101,21 @@ def test_short_rows(dtype, V, shift):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V,shift", [(601, 31, 0), (700, 300, 1), (640, 1000, 63), (1800, 2049, 5), (1777, 8190, 3)])
+def test_many_short_rows(dtype, T, V, shift):
+    """More rows than run at once; rows of equal logits, masked ones, one that holds NaN."""
+    x, ids = make(T, V, dtype, V + T, 2, shift)
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x[100:300].masked_fill_(torch.rand(200, V, device=DEV, generator=g) < 0.95, -INF)
+    x[300:310] = 1.5
+    x[310] = -INF
+    x[311, V // 2] = math.nan
+    x[400:600].copy_(torch.randint(-3, 4, (200, V), device=DEV, generator=g).to(dtype))
+    for k in (0, 5, 31):
+        check(_ops().token_logprobs(x, ids, top_k=k), reference(x, ids, k))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [40, 3001, 102400])
 def test_ties_and_order(dtype, V):
     """Equal logits, whole-number logits, rising and falling rows, -0.0 beside 0.0."""
