@@ -2,6 +2,7 @@
 // stream (so it can be captured into a CUDA graph) and checks the device, dtype
 // and contiguity assumptions of its kernel before launching.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -1090,6 +1091,11 @@ void ep_advance(const Tensor& epoch) {
 }
 
 // ---- log probabilities and shared cache pages
+// Their calls are as short as their tensors' allocation, so these come from the CUDA allocator
+// without a dispatch each (token_logprobs of one row 6.9 us of the host's time, 7.7 with at::empty).
+Tensor empty_f32(at::IntArrayRef size, c10::Device d) { return at::detail::empty_cuda(size, at::kFloat, d, c10::nullopt); }
+Tensor empty_i32(at::IntArrayRef size, c10::Device d) { return at::detail::empty_cuda(size, at::kInt, d, c10::nullopt); }
+
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& ids, int64_t k) {
   TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
               "token_logprobs: logits must be [T, V] with unit column stride");
@@ -1108,9 +1114,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
               "token_logprobs: top_k must be between 0 and min(" + std::to_string(sp::kLogprobsMaxTop) + ", V)");
   CHECK_CUDA(logits); CHECK_ON(logits, ids);
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
-  const Tensor lp = at::empty(ids.sizes(), f32), entropy = at::empty({T}, f32), top_lp = at::empty({T, k}, f32),
-               top_ids = at::empty({T, k}, ids.options());
+  const c10::Device d = logits.device();
+  const Tensor lp = empty_f32(ids.sizes(), d), entropy = empty_f32({T}, d), top_lp = empty_f32({T, k}, d),
+               top_ids = empty_i32({T, k}, d);
   sp::token_logprobs(logits.data_ptr(), st == at::kBFloat16 ? 0 : st == at::kHalf ? 1 : 2, logits.stride(0), (int)T,
                      (int)V, ids.data_ptr<int>(), (int)given, (int)k, num_sms(), lp.data_ptr<float>(),
                      entropy.data_ptr<float>(), top_lp.data_ptr<float>(), top_ids.data_ptr<int>(),
@@ -1133,11 +1139,10 @@ std::tuple<Tensor, Tensor> linear_logprobs(const Tensor& x, const Tensor& w, con
   TORCH_CHECK(T <= INT_MAX / 4 && V <= INT_MAX / 4 && K <= INT_MAX / 4, "linear_logprobs: too large");
   CHECK_CUDA(x); CHECK_ON(x, w); CHECK_ON(x, ids);
   const c10::cuda::CUDAGuard guard(x.device());
-  const auto f32 = x.options().dtype(at::kFloat);
-  const Tensor lp = at::empty({T}, f32), entropy = at::empty({T}, f32);
+  const Tensor lp = empty_f32({T}, x.device()), entropy = empty_f32({T}, x.device());
   if (T == 0) return {lp, entropy};
   const sp::LmPlan plan = sp::lm_plan((int)T, (int)V, (int)K, num_sms());
-  const Tensor work = at::empty({4 * plan.workspace()}, f32);
+  const Tensor work = empty_f32({4 * plan.workspace()}, x.device());
   sp::lm_logprobs(plan, x.data_ptr(), T > 1 ? x.stride(0) : (K + 7) / 8 * 8, w.data_ptr(), V > 1 ? w.stride(0) : (K + 7) / 8 * 8,
                   (int)T, (int)V, (int)K, ids.data_ptr<int>(), work.data_ptr(), lp.data_ptr<float>(),
                   entropy.data_ptr<float>(), err_word(), num_sms(), stream());
@@ -1197,7 +1202,7 @@ int64_t copy_pages(const Tensor& data, const c10::optional<Tensor>& scales, cons
   const int64_t n = src.numel();
   if (n == 0 || data.numel() == 0) return 0;
   const c10::cuda::CUDAGuard guard(data.device());
-  const Tensor work = at::empty({3 * n + 1}, src.options());
+  const Tensor work = empty_i32({3 * n + 1}, data.device());
   int* w = work.data_ptr<int>();
   sp::pages_pairs(src.data_ptr<int>(), dst.data_ptr<int>(), (int)n, (int)pages, (int)block_size, w + 1, w, err_word(),
                   stream());
@@ -1216,7 +1221,7 @@ std::tuple<Tensor, Tensor> fork_pages(const Tensor& table, const Tensor& lens, c
   CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, parents); CHECK_ON(table, refs);
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t n = parents.numel(), cols = table.size(1);
-  const Tensor new_table = at::empty({n, cols}, table.options()), new_lens = at::empty({n}, table.options());
+  const Tensor new_table = empty_i32({n, cols}, table.device()), new_lens = empty_i32({n}, table.device());
   sp::pages_fork(table.data_ptr<int>(), (int)table.size(0), (int)cols, lens.data_ptr<int>(), parents.data_ptr<int>(),
                  (int)n, refs.data_ptr<int>(), (int)refs.numel(), (int)block_size, new_table.data_ptr<int>(),
                  new_lens.data_ptr<int>(), stream());
@@ -1242,9 +1247,9 @@ Tensor reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs
   }
   CHECK_CUDA(table); CHECK_ON(table, lens); CHECK_ON(table, refs); CHECK_ON(table, data);
   const c10::cuda::CUDAGuard guard(table.device());
-  const Tensor short_by = at::empty({rows}, table.options());
+  const Tensor short_by = empty_i32({rows}, table.device());
   if (rows == 0) return short_by;
-  const Tensor work = at::empty({1 + 3 * rows + refs.numel()}, table.options());
+  const Tensor work = empty_i32({1 + 3 * rows + refs.numel()}, table.device());
   int* w = work.data_ptr<int>();
   sp::pages_reserve(table.data_ptr<int>(), (int)rows, (int)table.size(1), lens.data_ptr<int>(),
                     row_tokens.has_value() ? row_tokens->data_ptr<int>() : nullptr, (int)tokens,
@@ -1280,8 +1285,8 @@ std::tuple<Tensor, Tensor> compact_pages(const Tensor& table, const Tensor& refs
   CHECK_CUDA(table); CHECK_ON(table, refs); CHECK_ON(table, data);
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t n = refs.numel();
-  const Tensor page_map = at::empty({n}, refs.options()), live = at::empty({1}, refs.options());
-  const Tensor work = at::empty({1 + 4 * n}, table.options());
+  const Tensor page_map = empty_i32({n}, table.device()), live = empty_i32({1}, table.device());
+  const Tensor work = empty_i32({1 + 4 * n}, table.device());
   int* w = work.data_ptr<int>();
   sp::pages_compact(refs.data_ptr<int>(), (int)n, (int)block_size, page_map.data_ptr<int>(), live.data_ptr<int>(),
                     w + 1, w + 1 + 3 * n, w, stream());
