@@ -152,12 +152,13 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   tails[b] = tail;
   __syncthreads();
   bool leaves = false;
-  if (tail >= 0 && counts[tail] > 1) {
+  const int holders = tail >= 0 ? counts[tail] : 0;  // before any row's change: in large caches `counts` is refs itself
+  if (holders > 1) {
     // the rows before this one with the same last page will have left it
     int earlier = 0;
 #pragma unroll 8
     for (int q = 0; q < b; ++q) earlier += tails[q] == tail;
-    leaves = counts[tail] - earlier > 1;
+    leaves = holders - earlier > 1;
   }
   const int need = fresh + leaves;
   int all, total;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   unserved[b] = need > 0 && !served;
   __syncthreads();
   int lacks = served ? 0 : need;
-  if (all > found && need == 0 && tail >= 0 && counts[tail] > 1) {
+  if (all > found && need == 0 && holders > 1) {
     // a row that was to keep the page must not write to it while an earlier one is still there
     for (int q = 0; q < b; ++q)
       if (tails[q] == tail && unserved[q]) lacks = 1;

@@ -350,3 +350,28 @@ def test_captured_beam_steps():
         assert short.cpu().tolist() == want
         assert lens.cpu().tolist() == m.lens
         same(m, table, refs, data, None, "replay")
+
+
+@pytest.mark.parametrize("pages", [8192, 8193, 20000])
+def test_no_page_left_in_a_large_cache(pages):
+    """Pages run out among 1,000 rows that share last pages, with the counts in shared memory and read from
+    refs: what a row lacks goes by the counts before the call, not by what other rows changed meanwhile."""
+    ops = _ops()
+    rows, bs = 1000, 4
+    rng = random.Random(pages)
+    shared = rng.sample(range(pages), 250)  # four rows to a page, of one to three tokens
+    t = [[p] for p in shared for _ in range(4)]
+    n = [rng.randrange(1, bs) for _ in range(rows)]
+    r = [1] * pages
+    for p in shared:
+        r[p] = 4
+    for p in rng.sample([p for p in range(pages) if p not in set(shared)], 400):  # 400 pages for 750 rows that leave
+        r[p] = 0
+    for _ in range(5):
+        data = torch.randn(1, pages * bs, 2, device=DEV)
+        m = Model(t, n, r, [data.cpu()], bs)
+        table, lens, refs = ints(t), ints(n), ints(r)
+        short = ops.reserve_pages(table, lens, refs, data, 1, block_size=bs)
+        want = m.reserve(1)
+        assert sum(want) > 0 and short.cpu().tolist() == want
+        same(m, table, refs, data, None, pages)
