@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <stdexcept>
 
 #include "common.cuh"
@@ -114,11 +115,14 @@ void pages_fork(const int* table, int rows, int cols, const int* lens, const int
 // kNearRefs pages and up to kGrants granted pages stay in shared memory, so that a beam step
 // pays two dependent reads of memory (a row's length, its last page); larger caches read
 // refs again, larger grants go through `free_list` [pages]. `work` gets the copy list, (source,
-// destination, tokens) records, and `copies` its length.
+// destination, tokens) records, and `copies` its length. A row whose partly filled last page is
+// missing, and with `strict` one whose tokens go past the table's width, cannot be served: it
+// stays as it is, a holder of its pages like any idle row.
 __global__ void __launch_bounds__(kPagesMaxRows)
     pages_reserve_kernel(int* __restrict__ table, int rows, int cols, const int* __restrict__ lens,
-                         const int* __restrict__ row_tokens, int tokens, int* refs, int pages, int block_size,
-                         int* free_list, int* __restrict__ work, int* __restrict__ copies, int* __restrict__ short_by) {
+                         const int* __restrict__ row_tokens, int tokens, int strict, int* refs, int pages,
+                         int block_size, int* free_list, int* __restrict__ work, int* __restrict__ copies,
+                         int* __restrict__ short_by) {
   extern __shared__ int smem[];
   int* grants = smem;           // [kGrants]
   int* near = grants + kGrants; // [min(pages, kNearRefs)]
@@ -134,6 +138,7 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   if (b == 0) s_copies = 0;
   int* t = table + (long long)b * cols;
   int len = 0, want = 0, tail = -1, first = 0, last = 0, fresh = 0;
+  int lacks = 0;  // pages that the row lacks
   if (b < rows) {
     len = max(lens[b], 0);
     want = row_tokens ? row_tokens[b] : (len > 0 ? tokens : 0);
@@ -143,16 +148,24 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   if (want > 0) {
     if (len % block_size != 0 && len / block_size < cols) {
       tail = t[len / block_size];
-      if (tail < 0 || tail >= pages) tail = -1;
+      if (tail < 0 || tail >= pages) lacks = 1;
     }
     first = pages_of(len, block_size);
-    last = int(min((long long)cols, ((long long)len + want - 1) / block_size + 1));
+    const long long end = ((long long)len + want - 1) / block_size + 1;
+    last = int(min((long long)cols, end));
     for (int c = first; c < last; ++c) fresh += t[c] < 0;
+    if (strict && end > cols) lacks += int(min(end - cols, (long long)INT_MAX / 2));
+    if (lacks > 0) {
+      lacks += fresh;
+      tail = -1;
+      fresh = 0;
+    }
   }
   tails[b] = tail;
   __syncthreads();
   bool leaves = false;
-  const int holders = tail >= 0 ? counts[tail] : 0;  // before any row's change: in large caches `counts` is refs itself
+  // before any row's change: in large caches `counts` is refs itself
+  const int holders = tail >= 0 ? counts[tail] : 0;
   if (holders > 1) {
     // the rows before this one with the same last page will have left it
     int earlier = 0;
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   const bool served = start + need <= found;
   unserved[b] = need > 0 && !served;
   __syncthreads();
-  int lacks = served ? 0 : need;
+  if (!served) lacks += need;  // of a row that cannot be served need is 0
   if (all > found && need == 0 && holders > 1) {
     // a row that was to keep the page must not write to it while an earlier one is still there
     for (int q = 0; q < b; ++q)
@@ -208,14 +221,15 @@ __global__ void __launch_bounds__(kPagesMaxRows)
   if (b == 0) *copies = s_copies;
 }
 
-void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, int* refs,
-                   int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s) {
+void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, bool strict,
+                   int* refs, int pages, int block_size, int* free_list, int* work, int* copies, int* short_by,
+                   cudaStream_t s) {
   if (rows <= 0) return;
   if (rows > kPagesMaxRows) throw std::runtime_error("pages_reserve: too many rows");
   set_smem_bytes(pages_reserve_kernel, (int)sizeof(int) * (kGrants + kNearRefs));
   launch_k(pages_reserve_kernel, dim3(1), dim3(kPagesMaxRows),
            sizeof(int) * (kGrants + (pages <= kNearRefs ? pages : 0)), s, table, rows, cols, lens, row_tokens, tokens,
-           refs, pages, block_size, free_list, work, copies, short_by);
+           strict ? 1 : 0, refs, pages, block_size, free_list, work, copies, short_by);
 }
 
 // ------------------------------------------------------------------ free

@@ -350,8 +350,8 @@ struct PagePlane {
 };
 void pages_fork(const int* table, int rows, int cols, const int* lens, const int* parents, int n, int* refs, int pages,
                 int block_size, int* new_table, int* new_lens, cudaStream_t s);
-void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, int* refs,
-                   int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s);
+void pages_reserve(int* table, int rows, int cols, const int* lens, const int* row_tokens, int tokens, bool strict,
+                   int* refs, int pages, int block_size, int* free_list, int* work, int* copies, int* short_by, cudaStream_t s);
 void pages_free(int* table, int rows, int cols, int* refs, int pages, const int* which, int n, cudaStream_t s);
 void pages_compact(int* refs, int pages, int block_size, int* page_map, int* live, int* work, int* holes, int* copies,
                    cudaStream_t s);

@@ -1230,7 +1230,7 @@ std::tuple<Tensor, Tensor> fork_pages(const Tensor& table, const Tensor& lens, c
 
 Tensor reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& data,
                      const c10::optional<Tensor>& scales, const c10::optional<Tensor>& row_tokens, int64_t tokens,
-                     int64_t block_size) {
+                     int64_t block_size, bool strict) {
   check_page_table(table, refs, "reserve_pages");
   const int64_t rows = table.size(0);
   CHECK_I32(lens); CHECK_CONTIG(lens);
@@ -1252,7 +1252,7 @@ Tensor reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs
   const Tensor work = empty_i32({1 + 3 * rows + refs.numel()}, table.device());
   int* w = work.data_ptr<int>();
   sp::pages_reserve(table.data_ptr<int>(), (int)rows, (int)table.size(1), lens.data_ptr<int>(),
-                    row_tokens.has_value() ? row_tokens->data_ptr<int>() : nullptr, (int)tokens,
+                    row_tokens.has_value() ? row_tokens->data_ptr<int>() : nullptr, (int)tokens, strict,
                     refs.data_ptr<int>(), (int)refs.numel(), (int)block_size, w + 1 + 3 * rows, w + 1, w,
                     short_by.data_ptr<int>(), stream());
   sp::pages_copy(a, b, (int)data.size(0), (int)block_size, w + 1, w, std::min<int64_t>(rows, refs.numel()), nullptr, 0,

@@ -664,7 +664,7 @@ def fork_pages(block_table, lens, parents, refs, block_size=64):
     return out
 
 
-def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, cache_scales=None):
+def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, cache_scales=None, strict=False):
     """Room for ``tokens`` more tokens in every row, in place: missing pages behind lens[b]
     are the lowest free ones, and a partly filled last page that other rows hold too is
     replaced by a private copy of the row's tokens in it (every layer of the cache).
@@ -672,11 +672,15 @@ def reserve_pages(block_table, lens, refs, cache_data, tokens=1, block_size=64, 
     ``tokens``: a number (rows with lens[b] <= 0 are idle and get nothing) or int32 [rows].
     Rows are served in order, each wholly or not at all; of the rows that share a last page
     the last one keeps it, once the others have left. Returns int32 [rows], the pages that a
-    row lacks (0: it may be written). The table's width bounds a row; pages that a row has
+    row lacks. 0: its tokens have their pages, as far as the table is wide. With ``strict`` a
+    row whose tokens go past the table's width gets nothing and lacks the pages behind it too,
+    so that 0 says that all of them may be written; without, the caller keeps lens[b] + tokens
+    within columns * block_size (``paged_slots`` gives a position behind that slot 0). A row
+    whose partly filled last page is missing gets nothing and lacks it. Pages that a row has
     behind its last token are taken to be its own. At most PAGES_MAX_ROWS (1,024) rows."""
     per_row = tokens if isinstance(tokens, torch.Tensor) else None
     short = kernels().reserve_pages(block_table, lens, refs, cache_data, cache_scales, per_row,
-                                    0 if per_row is not None else int(tokens), int(block_size))
+                                    0 if per_row is not None else int(tokens), int(block_size), bool(strict))
     _count((1 + (cache_data.numel() > 0)) if block_table.shape[0] else 0)
     return short
 
@@ -790,7 +794,8 @@ def clear_status() -> None:
 # ------------------------------------------------------------------ DSA sparse attention
 def paged_slots(block_table, lens, rows, positions=None, block_size=64):
     """Cache slot of positions [0, lens[b]) (or of ``positions[b, :lens[b]]``) of each
-    sequence through its block table, [B, rows] int32 (slot 0 past the length)."""
+    sequence through its block table, [B, rows] int32 (slot 0 past the length, and for a
+    position outside the table's columns)."""
     B = block_table.shape[0]
     slots = torch.empty(B, rows, dtype=torch.int32, device=block_table.device)
     kernels().paged_slots(block_table, lens, positions, int(rows), int(block_size), slots)

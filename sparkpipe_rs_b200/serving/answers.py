@@ -58,7 +58,7 @@ class ParallelAnswers:
 
     def _reserve(self, tokens):
         return ops.reserve_pages(self.table, self.lens, self.refs, self.cache.data, tokens,
-                                 block_size=self.cache.block_size, cache_scales=self.cache.scales)
+                                 block_size=self.cache.block_size, cache_scales=self.cache.scales, strict=True)
 
     def _prefill(self, prompt) -> torch.Tensor:
         """Caches the prompt in row 0; returns the logits of its last token [1, V]."""

@@ -375,3 +375,92 @@ def test_no_page_left_in_a_large_cache(pages):
         want = m.reserve(1)
         assert sum(want) > 0 and short.cpu().tolist() == want
         same(m, table, refs, data, None, pages)
+
+
+class CheckedModel(Model):
+    """Reserves like Model, but leaves rows alone whose partly filled last page is missing, and with `strict`
+    those whose tokens go past the table's width."""
+
+    def reserve(self, tokens, strict=False):
+        want = list(tokens) if isinstance(tokens, list) else [tokens if n > 0 else 0 for n in self.lens]
+        lacks = [0] * len(self.table)
+        for b, row in enumerate(self.table):
+            n = max(self.lens[b], 0)
+            if want[b] <= 0:
+                continue
+            first, end = -(-n // self.bs), -(-(n + want[b]) // self.bs)
+            lost = n % self.bs and n // self.bs < len(row) and not self.held(row[n // self.bs])
+            past = max(0, end - len(row)) if strict else 0
+            if lost or past:
+                lacks[b] = bool(lost) + past + sum(e < 0 for e in row[first:end])
+                want[b] = 0
+        return [a + b for a, b in zip(super().reserve(want), lacks)]
+
+
+def test_no_room_in_the_table():
+    """Rows whose tokens go past the table's width: with `strict` each gets nothing and lacks what it would need,
+    the rows around them are served, and one that shares a page with such a row leaves it."""
+    ops = _ops()
+    bs, pages = 4, 12
+    t = [[0, 1], [2, 3], [4, 5], [6, -1], [7, 5]]
+    n, tokens = [8, 7, 6, 4, 5], [1, 2, 2, 9, 1]  # full; straddling; fits (shared page); fits in no table; fits
+    n[1], t[1] = 6, [2, 5]
+    tokens[1] = 5                                  # holds page 5 as well, and goes past the width
+    r = [0] * pages
+    for row in t:
+        for e in row:
+            if e >= 0:
+                r[e] += 1
+    data = torch.randn(2, pages * bs, 2, device=DEV)
+    m = CheckedModel(t, n, r, [data.cpu()], bs)
+    table, lens, refs = ints(t), ints(n), ints(r)
+    short = ops.reserve_pages(table, lens, refs, data, ints(tokens), block_size=bs, strict=True)
+    assert short.tolist() == [1, 1, 0, 3, 0]
+    assert table.tolist() == [[0, 1], [2, 5], [4, 3], [6, -1], [7, 8]] and refs.tolist()[5] == 1
+    assert m.reserve(tokens, True) == short.tolist()
+    same(m, table, refs, data, None, "strict")
+    one = ops.reserve_pages(ints([[0, 1]]), ints([2**31 - 1]), refs, data, 2**31 - 1, block_size=1, strict=True)
+    assert int(one) == 2**30 - 1  # 2^32 - 4 pages past the width, as many as are counted
+    # without it the width bounds a row
+    assert ops.reserve_pages(ints([[0, 1]]), ints([8]), ints(r), data, 1, block_size=bs).tolist() == [0]
+
+
+def test_last_page_missing():
+    """A row of some tokens whose last page is not there, or is no page of the cache, may not be written."""
+    ops = _ops()
+    bs = 4
+    t, n = [[0, -1, -1], [1, 99, -1], [2, 3, -1], [-1, -1, -1]], [6, 5, 7, 0]
+    r = [1, 1, 1, 1, 0, 0, 0, 0, 0]
+    for tokens, lacks in ((1, [1, 1, 0, 0]), (5, [2, 2, 0, 0])):
+        data = torch.randn(1, 9 * bs, 2, device=DEV)
+        m = CheckedModel(t, n, r, [data.cpu()], bs)
+        table, refs = ints(t), ints(r)
+        short = ops.reserve_pages(table, ints(n), refs, data, tokens, block_size=bs)
+        assert short.tolist() == lacks == m.reserve(tokens)
+        same(m, table, refs, data, None, tokens)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("rows,cols,pages,bs,layers", [(1, 1, 3, 1, 1), (5, 2, 9, 4, 2), (33, 3, 90, 16, 2),
+                                                       (200, 3, 9000, 3, 1)])
+def test_strict_rounds(kind, rows, cols, pages, bs, layers):
+    """Tables too narrow for many of their rows, pages that run out in some rounds, lengths past the width."""
+    ops = _ops()
+    rng = random.Random(rows + pages)
+    for _ in range(6):
+        t, n, r = random_state(rng, rows, cols, pages, bs)
+        for b in range(0, rows, 9):  # a last page that is lost, a length that the table does not hold
+            c = n[b] // bs
+            if n[b] % bs and c < cols and rng.random() < 0.5:
+                r[t[b][c]] -= 1
+                t[b][c] = -1
+            elif rng.random() < 0.3:
+                n[b] = cols * bs + rng.randrange(3 * bs)
+        data, scales = make_cache(kind, layers, pages, bs, rows)
+        m = CheckedModel(t, n, r, [p.cpu() for p in planes(data, scales)], bs)
+        tokens = [rng.choice([0, -1, 1, 1, bs, 2 * bs + 1]) for _ in range(rows)]
+        table, refs = ints(t).view(rows, cols), ints(r)
+        short = ops.reserve_pages(table, ints(n), refs, data, ints(tokens), block_size=bs, cache_scales=scales, strict=True)
+        assert short.cpu().tolist() == m.reserve(tokens, True)
+        same(m, table, refs, data, scales, "strict")
+    assert ops.status_word() == 0
