@@ -486,6 +486,18 @@ __global__ void __launch_bounds__(kCopyThreads)
   }
 }
 
+// Pieces of a first plane's page, about equal ones: a 73,728-byte page in four of a whole stage. A
+// plane whose pages are not all 16-byte aligned is copied by words, a page at a time.
+static int page_pieces(const PagePlane& p, int block_size) {
+  const int page_bytes = p.token_bytes * block_size;
+  const bool wide = ((reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.layer_stride | (uintptr_t)page_bytes) & 15) == 0;
+  return wide ? (page_bytes + kStageBytes - 1) / kStageBytes : 0;
+}
+
+bool pages_copy_fits(const PagePlane& a, int layers, int block_size, long long max_copies) {
+  return max_copies * layers * std::max(1, page_pieces(a, block_size)) < (1ll << 30);
+}
+
 void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_size, const int* work, const int* copies,
                 long long max_copies, int* table, long long entries, const int* page_map, int pages, int* err,
                 int num_sms, cudaStream_t s) {
@@ -493,12 +505,9 @@ void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_si
     return CopyPlane{static_cast<char*>(p.base), p.layer_stride, p.token_bytes * block_size, p.token_bytes};
   };
   const CopyPlane ca = plane(a), cb = plane(b);
-  const bool wide = ((reinterpret_cast<uintptr_t>(a.base) | (uintptr_t)a.layer_stride | (uintptr_t)ca.page_bytes) & 15) == 0;
-  // pieces of about equal size: a 73,728-byte page in three of a whole stage
-  const int pieces = wide ? (ca.page_bytes + kStageBytes - 1) / kStageBytes : 1;
+  const int wide = page_pieces(a, block_size), pieces = std::max(1, wide);
   const int piece_bytes = ((ca.page_bytes + pieces - 1) / pieces + 15) / 16 * 16;
   const long long units = max_copies * layers * pieces;
-  if (units >= (1ll << 30)) throw std::runtime_error("pages: too many pieces to copy in one call");
   const long long want = std::max(units, table ? (entries + kCopyThreads - 1) / kCopyThreads : 0ll);
   if (want <= 0) return;
   if (wide) {

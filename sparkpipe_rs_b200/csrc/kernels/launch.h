@@ -357,6 +357,9 @@ void pages_compact(int* refs, int pages, int block_size, int* page_map, int* liv
                    cudaStream_t s);
 void pages_pairs(const int* src, const int* dst, int n, int pages, int block_size, int* work, int* copies, int* err,
                  cudaStream_t s);
+// Whether `max_copies` pages of every layer are few enough for one pages_copy call (its units are
+// counted in 31 bits); asked before the index kernels change anything.
+bool pages_copy_fits(const PagePlane& a, int layers, int block_size, long long max_copies);
 void pages_copy(const PagePlane& a, const PagePlane& b, int layers, int block_size, const int* work, const int* copies,
                 long long max_copies, int* table, long long entries, const int* page_map, int pages, int* err,
                 int num_sms, cudaStream_t s);

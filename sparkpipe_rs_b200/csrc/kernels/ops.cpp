@@ -1167,9 +1167,9 @@ sp::PagePlane page_plane(const Tensor& t, int64_t block_size, const char* who) {
   return p;
 }
 
-// Both planes of a cache; returns its pages.
-int64_t page_planes(const Tensor& data, const c10::optional<Tensor>& scales, int64_t block_size, sp::PagePlane* a,
-                    sp::PagePlane* b, const char* who) {
+// Both planes of a cache, of which a call copies up to `copies` pages (and no more than there are); returns its pages.
+int64_t page_planes(const Tensor& data, const c10::optional<Tensor>& scales, int64_t block_size, int64_t copies,
+                    sp::PagePlane* a, sp::PagePlane* b, const char* who) {
   *a = page_plane(data, block_size, who);
   if (scales.has_value()) {
     TORCH_CHECK(scales->dim() == 3 && scales->size(0) == data.size(0) && scales->size(1) == data.size(1),
@@ -1179,6 +1179,8 @@ int64_t page_planes(const Tensor& data, const c10::optional<Tensor>& scales, int
   }
   const int64_t pages = data.size(1) / block_size;
   TORCH_CHECK(pages <= sp::kPagesMaxMarked && data.size(0) <= INT_MAX, who, ": too many pages");
+  TORCH_CHECK(sp::pages_copy_fits(*a, (int)data.size(0), (int)block_size, std::min(copies, pages)), who,
+              ": too many pieces to copy in one call");
   return pages;
 }
 
@@ -1197,7 +1199,7 @@ int64_t copy_pages(const Tensor& data, const c10::optional<Tensor>& scales, cons
   CHECK_I32(src); CHECK_I32(dst); CHECK_CONTIG(src); CHECK_CONTIG(dst);
   TORCH_CHECK(src.dim() == 1 && dst.dim() == 1 && src.numel() == dst.numel() && src.numel() <= INT_MAX / 3,
               "copy_pages: src and dst must be [n], a source for every destination");
-  const int64_t pages = page_planes(data, scales, block_size, &a, &b, "copy_pages");
+  const int64_t pages = page_planes(data, scales, block_size, src.numel(), &a, &b, "copy_pages");
   CHECK_CUDA(data); CHECK_ON(data, src); CHECK_ON(data, dst);
   const int64_t n = src.numel();
   if (n == 0 || data.numel() == 0) return 0;
@@ -1238,7 +1240,7 @@ Tensor reserve_pages(const Tensor& table, const Tensor& lens, const Tensor& refs
   TORCH_CHECK(rows <= sp::kPagesMaxRows, "reserve_pages: at most " + std::to_string(sp::kPagesMaxRows) + " rows");
   TORCH_CHECK(tokens >= 0 && tokens <= INT_MAX, "reserve_pages: tokens must not be negative");
   sp::PagePlane a, b;
-  const int64_t pages = page_planes(data, scales, block_size, &a, &b, "reserve_pages");
+  const int64_t pages = page_planes(data, scales, block_size, rows, &a, &b, "reserve_pages");
   TORCH_CHECK(refs.numel() <= pages, "reserve_pages: refs counts more pages than the cache has");
   if (row_tokens.has_value()) {
     CHECK_I32(*row_tokens); CHECK_CONTIG(*row_tokens);
@@ -1280,7 +1282,7 @@ std::tuple<Tensor, Tensor> compact_pages(const Tensor& table, const Tensor& refs
                                          const c10::optional<Tensor>& scales, int64_t block_size) {
   check_page_table(table, refs, "compact_pages");
   sp::PagePlane a, b;
-  const int64_t pages = page_planes(data, scales, block_size, &a, &b, "compact_pages");
+  const int64_t pages = page_planes(data, scales, block_size, refs.numel() / 2, &a, &b, "compact_pages");
   TORCH_CHECK(refs.numel() <= pages, "compact_pages: refs counts more pages than the cache has");
   CHECK_CUDA(table); CHECK_ON(table, refs); CHECK_ON(table, data);
   const c10::cuda::CUDAGuard guard(table.device());

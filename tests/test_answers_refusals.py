@@ -112,3 +112,20 @@ def test_free_and_compact():
     for refs, says in ((i32(3), "more pages than the cache"), (i32(2), "CUDA")):
         with pytest.raises((ValueError, RuntimeError), match=says):
             ops.compact_pages(i32(3, 4), refs, CACHE)
+
+
+def test_too_many_pieces():
+    """Caches of more pieces than one call counts are refused before an index kernel changes tables or counts."""
+    ops = _ops()
+    n = 1 << 20
+    data = torch.empty(2048, n, 4, dtype=torch.uint8, device="meta")  # 2,048 layers of a million 4-byte pages
+    with pytest.raises(RuntimeError, match="compact_pages: too many pieces"):
+        ops.compact_pages(i32(3, 4), i32(n), data, block_size=1)
+    with pytest.raises(RuntimeError, match="copy_pages: too many pieces"):
+        ops.copy_pages(data, i32(n // 2), i32(n // 2), block_size=1)
+    wide = torch.empty(1 << 20, 1024, 16, dtype=torch.uint8, device="meta")  # a million layers of 1,024 pages
+    with pytest.raises(RuntimeError, match="reserve_pages: too many pieces"):
+        ops.reserve_pages(i32(1024, 4), i32(1024), i32(1024), wide, block_size=1)
+    for few in (data[:2047], wide[:, :1023]):  # one layer, or one page, less
+        with pytest.raises(RuntimeError, match="CUDA"):
+            ops.copy_pages(few, i32(n // 2), i32(n // 2), block_size=1)
