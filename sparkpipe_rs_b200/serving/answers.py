@@ -9,7 +9,7 @@ back (``ops.free_pages``) and the kept ones' pages move to the front of the cach
 (``ops.compact_pages``), where ``table`` / ``lens`` let a caller go on from them.
 
 Everything between the prefill and the ranking stays on the device; with stop tokens the
-host reads one flag per step.
+host reads two numbers per step.
 """
 from __future__ import annotations
 
@@ -45,6 +45,9 @@ class ParallelAnswers:
             raise ValueError(f"ParallelAnswers: the model's positions end at {model.cos_sin.shape[0]}")
         if getattr(model, "ep", None) is not None:
             raise ValueError("ParallelAnswers: one rank only")
+        most = min(ops.kernels().LOGPROBS_MAX_TOP, model.cfg.vocab_size)
+        if not 0 <= top_logprobs <= most:
+            raise ValueError(f"ParallelAnswers: 0 to {most} alternatives")
         self.model, self.cache, self.n = model, cache, answers
         self.cols = -(-max_tokens_per_row // cache.block_size)
         self.max_tokens = max_tokens_per_row
@@ -79,7 +82,9 @@ class ParallelAnswers:
     def generate(self, prompt, max_new_tokens: int, temperature: float = 1.0, seed: int = 0, keep: int = 1,
                  stop_token_ids: tuple = ()) -> list[Answer]:
         """The ``keep`` answers of the highest mean log probability, best first. Equal seeds
-        give equal answers; answer i draws with noise key seed * answers + i."""
+        give equal answers; answer i draws with noise key seed * answers + i. Too few pages for
+        the answers are a MemoryError: before the first step, or with stop tokens, which may end
+        answers sooner, within two steps of running out."""
         n, g, c = self.n, self.graph, self.cache
         if not 1 <= keep <= n:
             raise ValueError("ParallelAnswers: keep between 1 and the number of answers")
@@ -88,6 +93,11 @@ class ParallelAnswers:
         if not all(0 <= int(t) < self.model.cfg.vocab_size for t in prompt):
             raise ValueError("ParallelAnswers: token ids outside the vocabulary")
         logits = self._prefill(prompt)
+        P, bs = len(prompt), c.block_size
+        # the prompt's whole pages once, the rest per answer; the last token is not cached
+        pages = P // bs + n * (-(-(P + max_new_tokens - 1) // bs) - P // bs) if max_new_tokens > 1 else 0
+        if pages > c.num_blocks and not stop_token_ids:
+            raise MemoryError(f"ParallelAnswers: the cache ran out of pages: {pages} are needed, it has {c.num_blocks}")
         self.table, self.lens = ops.fork_pages(self.table, self.lens, torch.zeros(n, **self._i32), self.refs,
                                                block_size=c.block_size)
         temps = torch.full((n,), float(temperature), dtype=torch.float32, device=self.model.device)
@@ -105,7 +115,10 @@ class ParallelAnswers:
         for t in range(1, max_new_tokens):
             if stops is not None:
                 live = live & ~(tokens[:, None] == stops).any(1)
-                if not bool(live.any()):
+                any_live, lacking = torch.stack([live.sum(), short]).tolist()  # the step's one read
+                if lacking:
+                    raise MemoryError("ParallelAnswers: the cache ran out of pages")
+                if not any_live:
                     break
             ended.append(live)
             short = short + self._reserve(live.int()).sum()

@@ -173,3 +173,27 @@ def test_answers_refused(model):
     with pytest.raises(MemoryError, match="ran out"):
         pa.generate([1] * 100, 60)  # two pages of prompt, a copy of the second, and no third for both
     assert len(pa.generate([1] * 60, 3, keep=2)) == 2
+
+
+def test_answers_out_of_pages(model, monkeypatch):
+    """Too few pages end a call before its first step, or with stop tokens soon after the page is missing, and
+    not at the end of the answers; the next call starts afresh."""
+    pa, _ = _answers(model, 2, blocks=3)
+    steps = []
+    run = pa.graph.run
+    monkeypatch.setattr(pa.graph, "run", lambda: (steps.append(1), run())[1])
+    with pytest.raises(MemoryError, match="ran out"):
+        pa.generate([1] * 100, 200)
+    assert not steps
+    with pytest.raises(MemoryError, match="ran out"):
+        pa.generate([1] * 100, 200, stop_token_ids=(-2,))
+    assert 28 <= len(steps) <= 30  # tokens 100 to 127 fit, the third page of both rows does not
+    for plen, new, fits in ((100, 29, True), (100, 30, False), (64, 65, True), (64, 66, False), (128, 1, True)):
+        if fits:
+            assert [len(a.token_ids) for a in pa.generate([1] * plen, new, keep=2)] == [new, new]
+            continue
+        with pytest.raises(MemoryError, match="ran out"):
+            pa.generate([1] * plen, new, keep=2)
+    for top in (-1, 33):
+        with pytest.raises(ValueError, match="alternatives"):
+            type(pa)(model, pa.cache, 2, 320, top_logprobs=top)
