@@ -129,3 +129,13 @@ def test_too_many_pieces():
     for few in (data[:2047], wide[:, :1023]):  # one layer, or one page, less
         with pytest.raises(RuntimeError, match="CUDA"):
             ops.copy_pages(few, i32(n // 2), i32(n // 2), block_size=1)
+
+
+def test_engine_config_order():
+    """A setting that came later stands last: those before it keep their places."""
+    from dataclasses import fields
+
+    from sparkpipe_rs_b200.serving.engine import EngineConfig
+
+    names = [f.name for f in fields(EngineConfig)]
+    assert names[-1] == "logprobs" and names[names.index("warm_prefill") + 1] == "prefill_graphs"
