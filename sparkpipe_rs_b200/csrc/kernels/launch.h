@@ -333,6 +333,7 @@ void token_logprobs(const void* logits, int dtype, long long ld, int rows, int V
 constexpr int kLmRows = 128;  // rows of a CTA's tile
 struct LmPlan {
   int ctas = 1, row_tiles = 0, units = 0, shares = 1;
+  int segment = 0, per_stage = 0;  // K blocks (of 64) that are added up in one accumulator, and of a ring stage
   long long workspace() const { return 2ll * shares * row_tiles * ctas * kLmRows; }
 };
 LmPlan lm_plan(int T, int V, int K, int num_sms);

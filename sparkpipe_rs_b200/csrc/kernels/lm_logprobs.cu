@@ -29,7 +29,6 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
-#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -445,12 +444,31 @@ static LmPlan plan_as(int T, int V, int K, int num_sms, long long& cost) {
 // are finer and the last row tile's empty rows fewer (333 x 10,007 x 1,000 20 us, pairs 22; 300 x
 // 50,000 x 2,048 69 against 75). One row tile stays on single CTAs, whose shorter segments keep
 // the entropy within 2e-7 there.
-LmPlan lm_plan(int T, int V, int K, int num_sms) {
+static LmPlan best_shares(int T, int V, int K, int num_sms) {
   long long one = 0, two = 0;
   const LmPlan single = plan_as<1>(T, V, K, num_sms, one);
   if (T <= kRows || num_sms < 2) return single;
   const LmPlan pairs = plan_as<2>(T, V, K, num_sms, two);
   return two <= one ? pairs : single;
+}
+
+// Rows of a box of x. A few rows load only themselves (in swizzle atoms of 8): a CTA's copies move
+// about 55 GB/s in rows of 128 bytes, and x, read again for each tile, should not take a third of it.
+// The MMA's other rows are whatever shared memory held; theirs are results that nobody reads.
+static int x_rows(const LmPlan& l, int T) { return l.row_tiles * l.ctas == 1 ? (T + 7) / 8 * 8 : kRows; }
+static int block_bytes(const LmPlan& l, int T) {  // of x and of the boxes of the largest tile
+  const int boxes = std::min(kCols / (kBox * l.ctas), (l.units + l.shares - 1) / l.shares);
+  return x_rows(l, T) * kBlockK * 2 + boxes * kBoxBytes;
+}
+
+LmPlan lm_plan(int T, int V, int K, int num_sms) {
+  LmPlan l = best_shares(T, V, K, num_sms);
+  const bool many = l.ctas == 2 && V >= kManyTokens;
+  l.segment = many ? 16 : l.row_tiles > 1 || l.ctas == 2 ? 8 : 4;
+  // Stages of two K blocks where four fit: a narrow share's K block costs what its warps need to
+  // issue it, half of which is the stage's (9,472 tokens, 16 rows: 0.33 us a block, in twos 0.26).
+  l.per_stage = !many && 8 * block_bytes(l, T) <= kRing ? 2 : 1;
+  return l;
 }
 
 template <int CTAS, int SEG, int PER>
@@ -495,33 +513,20 @@ void lm_logprobs(const LmPlan& l, const void* x, long long ldx, const void* w, l
   p.ids = ids;
   p.part = static_cast<float4*>(workspace);
   p.err = err;
-  // A few rows load only themselves (in swizzle atoms of 8): a CTA's copies move about 55 GB/s
-  // in rows of 128 bytes, and x, read again for each tile, should not take a third of it. The
-  // MMA's other rows are whatever shared memory held; theirs are results that nobody reads.
-  const int x_rows = l.row_tiles * l.ctas == 1 ? (T + 7) / 8 * 8 : kRows;
-  p.x_bytes = x_rows * kBlockK * 2;
-  const int boxes = std::min(kCols / (kBox * l.ctas), (l.units + l.shares - 1) / l.shares);
-  p.block_bytes = p.x_bytes + boxes * kBoxBytes;
-  const bool many = l.ctas == 2 && V >= kManyTokens;
-  // Stages of two K blocks where four fit: a narrow share's K block costs what its warps need to
-  // issue it, half of which is the stage's (9,472 tokens, 16 rows: 0.33 us a block, in twos 0.26).
-  const int per = !many && 8 * p.block_bytes <= kRing ? 2 : 1;
+  p.x_bytes = x_rows(l, T) * kBlockK * 2;
+  p.block_bytes = block_bytes(l, T);
+  const int per = l.per_stage;
   p.stage_bytes = per * p.block_bytes;
   // the MMA reads 128 rows of x from the last block too, whatever a box holds
   const int behind = (per - 1) * p.block_bytes + std::max(p.block_bytes, kXBytes);
   p.stages = std::min(kMaxStages, (kRing - behind) / p.stage_bytes + 1);
   CUtensorMap tx, tw;
-  make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows, kBlockK);
+  make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, K, ldx, x_rows(l, T), kBlockK);
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
-  auto run = [&](auto two) {
-    constexpr int PER = decltype(two)::value ? 2 : 1;
-    if (l.ctas == 2) launch_lm<2, 8, PER>(l, tx, tw, p, num_sms, s);
-    else if (l.row_tiles > 1) launch_lm<1, 8, PER>(l, tx, tw, p, num_sms, s);
-    else launch_lm<1, 4, PER>(l, tx, tw, p, num_sms, s);
-  };
-  if (many) launch_lm<2, 16, 1>(l, tx, tw, p, num_sms, s);
-  else if (per == 2) run(std::true_type{});
-  else run(std::false_type{});
+  if (l.segment == 16) launch_lm<2, 16, 1>(l, tx, tw, p, num_sms, s);
+  else if (l.ctas == 2) per == 2 ? launch_lm<2, 8, 2>(l, tx, tw, p, num_sms, s) : launch_lm<2, 8, 1>(l, tx, tw, p, num_sms, s);
+  else if (l.segment == 8) per == 2 ? launch_lm<1, 8, 2>(l, tx, tw, p, num_sms, s) : launch_lm<1, 8, 1>(l, tx, tw, p, num_sms, s);
+  else per == 2 ? launch_lm<1, 4, 2>(l, tx, tw, p, num_sms, s) : launch_lm<1, 4, 1>(l, tx, tw, p, num_sms, s);
   launch_k(lm_logprobs_join_kernel, dim3(T), dim3(32), 0, s, (const float4*)workspace, 2 * p.shares,
            p.row_tiles * l.ctas * kRows, T, V, ids, lp, entropy);
 }

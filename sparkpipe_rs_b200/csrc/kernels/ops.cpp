@@ -1149,6 +1149,15 @@ std::tuple<Tensor, Tensor> linear_logprobs(const Tensor& x, const Tensor& w, con
   return {lp, entropy};
 }
 
+// How linear_logprobs would go about a problem: CTAs of a tile, K blocks of an accumulator's segment,
+// K blocks of a ring stage, row tiles, shares of the vocabulary.
+std::tuple<int, int, int, int, int> linear_logprobs_plan(int64_t T, int64_t V, int64_t K, int64_t sms) {
+  TORCH_CHECK(T >= 1 && V >= 1 && K >= 1 && sms >= 1 && T <= INT_MAX / 4 && V <= INT_MAX / 4 && K <= INT_MAX / 4 &&
+                  sms <= 4096, "linear_logprobs_plan: sizes");
+  const sp::LmPlan l = sp::lm_plan((int)T, (int)V, (int)K, (int)sms);
+  return {l.ctas, l.segment, l.per_stage, l.row_tiles, l.shares};
+}
+
 // One plane of a paged cache [layers, slots, row]; any layer stride, rows and slots dense.
 sp::PagePlane page_plane(const Tensor& t, int64_t block_size, const char* who) {
   TORCH_CHECK(t.dim() == 3 && t.size(2) >= 1 && (t.stride(2) == 1 || t.size(2) == 1) &&
@@ -1337,6 +1346,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_blocks_copy", &kv_blocks_copy);
   m.def("token_logprobs", &token_logprobs);
   m.def("linear_logprobs", &linear_logprobs);
+  m.def("linear_logprobs_plan", &linear_logprobs_plan);
   m.def("copy_pages", &copy_pages);
   m.def("fork_pages", &fork_pages);
   m.def("reserve_pages", &reserve_pages);
