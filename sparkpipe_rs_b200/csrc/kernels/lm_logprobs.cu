@@ -467,7 +467,8 @@ LmPlan lm_plan(int T, int V, int K, int num_sms) {
   l.segment = many ? 16 : l.row_tiles > 1 || l.ctas == 2 ? 8 : 4;
   // Stages of two K blocks where four fit: a narrow share's K block costs what its warps need to
   // issue it, half of which is the stage's (9,472 tokens, 16 rows: 0.33 us a block, in twos 0.26).
-  l.per_stage = !many && 8 * block_bytes(l, T) <= kRing ? 2 : 1;
+  // Single CTAs on several row tiles hold 128 rows of x and shares that are too wide for that.
+  l.per_stage = (l.ctas == 2 ? !many : l.segment == 4) && 8 * block_bytes(l, T) <= kRing ? 2 : 1;
   return l;
 }
 
@@ -525,7 +526,7 @@ void lm_logprobs(const LmPlan& l, const void* x, long long ldx, const void* w, l
   make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, V, K, ldw, kBox, kBlockK);
   if (l.segment == 16) launch_lm<2, 16, 1>(l, tx, tw, p, num_sms, s);
   else if (l.ctas == 2) per == 2 ? launch_lm<2, 8, 2>(l, tx, tw, p, num_sms, s) : launch_lm<2, 8, 1>(l, tx, tw, p, num_sms, s);
-  else if (l.segment == 8) per == 2 ? launch_lm<1, 8, 2>(l, tx, tw, p, num_sms, s) : launch_lm<1, 8, 1>(l, tx, tw, p, num_sms, s);
+  else if (l.segment == 8) launch_lm<1, 8, 1>(l, tx, tw, p, num_sms, s);
   else per == 2 ? launch_lm<1, 4, 2>(l, tx, tw, p, num_sms, s) : launch_lm<1, 4, 1>(l, tx, tw, p, num_sms, s);
   launch_k(lm_logprobs_join_kernel, dim3(T), dim3(32), 0, s, (const float4*)workspace, 2 * p.shares,
            p.row_tiles * l.ctas * kRows, T, V, ids, lp, entropy);
