@@ -327,10 +327,10 @@ __global__ void __launch_bounds__(64 + kEpilogue, 1)
         float s, t, e, f;
         unpack2(add2(s0, s1), s, t);
         unpack2(add2(e0, e1), e, f);
-        a.add(s + t, e + f);
+        a.add_long(s + t, e + f);
       }
       if (!ok) a.hi = NAN;
-      p.part[(long long)(share * 2 + half) * p.row_tiles * CTAS * kRows + row] = make_float4(a.m, a.hi + a.lo, a.e, given);
+      p.part[(long long)(share * 2 + half) * p.row_tiles * CTAS * kRows + row] = make_float4(a.m, a.hi + a.lo, a.e + a.el, given);
     }
   }
   if (CTAS == 2) cluster_sync();  // a pair's shared memory serves both CTAs

@@ -38,26 +38,37 @@ SP_DEVI float max_nan(float a, float b) {
   return r;
 }
 
-// Running sums of a thread: terms 2^u, u = (x - m) log2 e, in hi + lo, and terms 2^u u in e.
+// Running sums of a thread: terms 2^u, u = (x - m) log2 e, in hi + lo, and terms 2^u u in e, with
+// add_long in e + el.
 struct LogprobSums {
-  float m = -INFINITY, hi = 0.f, lo = 0.f, e = 0.f;
+  float m = -INFINITY, hi = 0.f, lo = 0.f, e = 0.f, el = 0.f;
 
   SP_DEVI void raise(float top) {  // a larger maximum
     if (top > m) {
       const float d = fmaxf((m - top) * kLog2e, -300.f);  // m = -inf: the sums are 0
       const float w = fast_exp2(d);
       e = w * fmaf(hi, d, e);
+      el *= w;
       hi *= w;
       lo *= w;
       m = top;
     }
   }
   SP_DEVI float shift() const { return m == -INFINITY ? 0.f : -m; }  // only -inf so far: u = -inf
+  // a + b in `a`, what its rounding leaves added to `low`
+  static SP_DEVI void keep(float& a, float& low, float b) {
+    const float t = a + b, z = t - a;
+    low += (a - (t - z)) + (b - z);
+    a = t;
+  }
   SP_DEVI void add(float s, float f) {
-    const float t = hi + s, z = t - hi;
-    lo += (hi - (t - z)) + (s - z);
-    hi = t;
+    keep(hi, lo, s);
     e += f;
+  }
+  // for hundreds of additions, whose roundings would show in the entropy
+  SP_DEVI void add_long(float s, float f) {
+    keep(hi, lo, s);
+    keep(e, el, f);
   }
 };
 

@@ -157,3 +157,19 @@ def test_graph_and_streams(T, V, K):
             assert torch.equal(out[0], want[i][0]) and torch.equal(out[1], want[i][1])
         assert torch.equal(beside[0], want[1][0]) and torch.equal(beside[1], want[1][1])
     assert ops.status_word() == 0
+
+
+def test_entropy_of_one_long_share():
+    """A thread's sums over all 640 tiles of a row, with the tiles' rounding errors kept: what is left is the rounding
+    of a part's E (2^-24 of it, E / S being 0.55 of the entropy here), of ln S (0.46 of it) and of the entropy, 2^-23
+    together, and with plain fp32 sums it was 2^-22.7."""
+    ops = _ops()
+    T, V, K, n = 18944, 163840, 64, 256
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(T, K, device=DEV, generator=g).bfloat16()
+    w = (torch.randn(V, K, device=DEV, generator=g) * 0.3125).bfloat16()
+    ids = torch.zeros(T, dtype=torch.int32, device=DEV)
+    ent = ops.linear_logprobs(x, w, ids)[1]
+    for rows in (slice(0, n), slice(T // 2, T // 2 + n), slice(T - n, T)):
+        want = reference(x[rows].double() @ w.double().t(), ids[rows])[1]
+        assert float((ent[rows].double() - want).norm() / want.norm()) < 2**-23
