@@ -400,7 +400,7 @@ SP_DEVI void bulk_store(void* dst, const void* src, uint32_t bytes) {
 
 // Units are (pair, layer, piece of the first plane), dealt to the CTAs in turn. One thread moves
 // them through a ring of shared memory with bulk copies: the load of a unit goes out while the
-// one before it is stored. The other warps move the second plane (block scales, a sixtieth
+// one before it is stored. The other warps move the second plane (block scales, a thirtieth
 // of the bytes) and what a token count leaves of 16 bytes. Pairs carry a token count because a
 // last page is copied as far as its row has tokens.
 __global__ void __launch_bounds__(kCopyThreads)

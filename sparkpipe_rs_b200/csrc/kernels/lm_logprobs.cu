@@ -14,11 +14,13 @@
 //    below its last bit instead of rounding: over long K the logits shrink by about 1e-6 of
 //    their size, all the same way, which shows in the entropy (off by 1.5e-6 of itself at K =
 //    2,048). So K is taken in segments, each with an accumulator of its own, and the epilogue
-//    adds the segments with rounding: segments of 512 (off by 3e-7 to 6e-7, the more the fewer
-//    tokens there are), of 256 where one row tile leaves the epilogue idle anyway (1.5e-7 to
-//    3e-7), but of 1,024 on CTA pairs over 32,768 tokens and more, where the power limit makes
-//    each pass of the epilogue cost 5% (8,192 x 102,400 x 2,048: 2.47 ms, off by 7e-7; 2.59 ms
-//    in segments of 512; one accumulator would be 2.5% faster still).
+//    adds the segments with rounding. Off from 64 bits (2-norm, logits of variance 6): segments
+//    of 512 3e-7 to 4.5e-7, of 256, where one row tile leaves the epilogue idle anyway, 1.2e-7 to
+//    1.7e-7 (a single row up to 2.4e-7), of 1,024 6e-7 to 1e-6, the less the more tokens there
+//    are. On CTA pairs each pass of the epilogue costs: segments of 1,024 are 5 to 9% faster than
+//    of 512 whatever the number of rows and tokens (150 x 32,768 x 2,048 34.8 us, 38.1; 8,192 x
+//    102,400 x 2,048 at the power limit 2.45 ms, 2.60; K = 7,168 0 to 4%). They are taken from 32,768 tokens on, where
+//    they keep the entropy within 9e-7 (10,000 tokens: 1e-6).
 //  * Work items are (128 rows, a range of 64-token units of the vocabulary), rows fastest:
 //    the CTAs that run at the same time read the same range of w, so it comes from memory
 //    once and then from L2, and one row tile's shares are few enough to join cheaply.
@@ -47,7 +49,7 @@ constexpr int kXBytes = kRows * kBlockK * 2;
 constexpr int kBoxBytes = kBox * kBlockK * 2;
 constexpr int kHalf = 128;       // columns of an epilogue thread
 constexpr int kEpilogue = 256;   // epilogue threads
-constexpr int kManyTokens = 32768;  // long segments of K from here on
+constexpr int kManyTokens = 32768;  // pairs take long segments of K from here on
 
 // CTAs = 2: a pair of CTAs shares a tile of 256 rows x 256 logits, each loads half of w's rows.
 template <int CTAS>
@@ -439,11 +441,10 @@ static LmPlan plan_as(int T, int V, int K, int num_sms, long long& cost) {
   return l;
 }
 
-// CTA pairs read half as much of w per SM (8,192 x 102,400 x 2,048 2.07 ms, single CTAs 2.83; 256
-// x 32,000 x 4,096 60 us against 71 to 87, 512 x 10,007 x 1,000 22 against 27), single CTAs' items
-// are finer and the last row tile's empty rows fewer (333 x 10,007 x 1,000 20 us, pairs 22; 300 x
-// 50,000 x 2,048 69 against 75). One row tile stays on single CTAs, whose shorter segments keep
-// the entropy within 2e-7 there.
+// CTA pairs read half as much of w per SM (8,192 x 102,400 x 2,048 2.27 ms in a short run, single CTAs on
+// the same card 2.56; 256 x 32,000 x 4,096 67 us against 72, 512 x 10,007 x 1,000 23 against 26), single CTAs' items
+// are finer and the last row tile's empty rows fewer (333 x 10,007 x 1,000 19 us, pairs 21; 300 x
+// 50,000 x 2,048 71 against 80). One row tile stays on single CTAs and their short segments.
 static LmPlan best_shares(int T, int V, int K, int num_sms) {
   long long one = 0, two = 0;
   const LmPlan single = plan_as<1>(T, V, K, num_sms, one);
